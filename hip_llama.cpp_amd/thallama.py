@@ -79,6 +79,16 @@ class Q8Checkpoint(C.Structure):
                 ("payload_bytes", C.c_size_t)]
 
 
+class Q8KVCache(C.Structure):
+    """include/thaDNN/thaDNN_q8_kv.hpp: an int8 K/V cache (device pointers and sizes)"""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ks", "vs")] + \
+               [(n, C.c_int) for n in ("n_batches", "n_layers", "n_kv_heads", "head_size", "seq_len", "block")]
+
+    @classmethod
+    def make(cls, n_batches, n_layers, n_kv_heads, head_size, seq_len, block, k=None, v=None, ks=None, vs=None):
+        return cls(k, v, ks, vs, n_batches, n_layers, n_kv_heads, head_size, seq_len, block)
+
+
 class Handle(C.Structure):
     """thablasHandle_t, reference include/thaBLAS.hpp:21-25"""
     _fields_ = [("current_gpu_id", C.c_int), ("calc_stream", C.c_void_p), ("copy_stream", C.c_void_p)]
@@ -152,6 +162,13 @@ def lib():
             "thaBLAS_q8_matmul_batch": (I, [C.POINTER(Handle), I, P, P, C.POINTER(C.c_int8), P, I, I, I, I, I]),
             "thaDNN_q8_forward_batch": (I, [Handle, I, C.POINTER(Config), C.POINTER(Q8TransformerWeights),
                                             C.POINTER(RunState), c_int_p, c_int_p, P]),
+            "thallama_q8_kv_bytes": (S, [I, I, I, I, I, I]),
+            "thallama_q8_kv_map": (I, [C.POINTER(Q8KVCache), VP, I, I, I, I, I, I]),
+            "thaDNN_q8_kv_store_batch": (I, [C.POINTER(Handle), C.POINTER(Q8KVCache), I, I, I, VP, VP, VP, VP, I]),
+            "thaDNN_q8_kv_load_batch": (I, [C.POINTER(Handle), C.POINTER(Q8KVCache), I, I, I, VP, VP, VP, VP, I]),
+            "thaDNN_q8_attention_workspace": (S, [C.POINTER(Q8KVCache), I, I, I]),
+            "thaDNN_q8_attention_batch": (I, [C.POINTER(Handle), C.POINTER(Q8KVCache), I, I, I, VP, VP, I, VP, VP, I, I,
+                                              VP, S]),
             "thallama_decoder_destroy": (None, [VP]),
             "thallama_decoder_set": (I, [VP, I, I]),
             "thallama_decoder_persistent": (I, [VP]),

@@ -7,6 +7,7 @@
 #include "thaDNN/thaDNN_mha.hpp"
 #include "thaDNN/thaDNN_softmax.hpp"
 #include "thaDNN/thaDNN_swiglu.hpp"
+#include "thaDNN/thaDNN_q8_kv.hpp"
 
 #include "utils.hpp"
 // the reference's thaDNN.hpp includes <omp.h> (its pipeline driver takes omp_lock_t*)
