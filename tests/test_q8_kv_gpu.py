@@ -288,17 +288,19 @@ def test_attention_values_of_very_different_size(gpu, handle, nt):
     pos = [S - nt] * B
     got = dev.attend(0, pos, None, q).reshape(q.shape)
     want, bound = ref.attend(0, pos, [nt] * B, nt, q, 1)
-    # the bound with the largest value is far above the last row's results: hold that one to its own size
     hold(got, want, bound, "different sizes")
-    size = np.abs(want[:, -1]).max()
-    u = 2.0 ** -24
+    # That bound goes by the largest value, far above what the last row gets: hold it to its own size.  A weight times
+    # its value block's scale, w_t = p_t sv_t, is held as n_t / 0x7f7f7f of 2^M with max w >= 2^M / 2, so it is off by
+    # at most half a step, 2^M 2^-24 (1 + 2^-7) <= 2^-22 max w, times a code of at most 127; beside that each term is off by
+    # its weight's own error, 2 (E + 8u |x|) + 32u of attend's bound and T u for each sum, all under 2^-15 here.
     for b in range(B):
         x = ref.values("k", 0, np.float64)[b, :, :pos[b] + nt] @ q[b, -1].astype(np.float64)[:, :, None] / 8.0
         e = np.exp(x - x.max(1, keepdims=True))
-        w = (e / e.sum(1, keepdims=True)) * np.abs(ref.values("v", 0, np.float64)[b, :, :pos[b] + nt])
-        # each weight is known to 2^-15 of itself, or to u of the largest weight times its value block's size
-        lim = 2.0 ** -15 * w.sum(1) + len(x[0]) * 4 * u * 127 * w.max(1).max(1, keepdims=True)
-        assert (np.abs(got[b, -1] - want[b, -1]) <= lim).all(), (b, size)
+        p = e / e.sum(1, keepdims=True)
+        w = p * np.repeat(ref.scales["v"][b, 0].astype(np.float64), block, -1)[:, :pos[b] + nt, None]
+        v = np.abs(ref.values("v", 0, np.float64)[b, :, :pos[b] + nt])
+        lim = 2.0 ** -15 * (p * v).sum(1) + x.shape[1] * 2.0 ** -22 * 127 * w.max(1)
+        assert (np.abs(got[b, -1] - want[b, -1]) <= lim).all(), b
 
 
 @pytest.mark.parametrize("nt", [1, 20])
