@@ -80,97 +80,103 @@ TL_DEVICE void digits4(const unsigned (&n)[4], int& p0, int& p1, int& p2) {
 
 TL_DEVICE i4 mfma(i4 a, i4 b, i4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
-// A wave's state for QT tiles of 16 query rows.  KS = steps of 64 dimensions.
-template <int KS, int QT>
-struct AttnWave {
-  static constexpr int DT = 4 * KS;  // value tiles of 16 dimensions
-  i4 q[QT][3][KS];                   // query digits, lowest first
-  int qe[QT];                        // their power of two
-  float qn[QT];                      // 1, or NaN for a query that is not finite
-  int seen[QT];                      // keys that the row sees
-  float M[QT], sum[QT];
-  f4 o[QT][DT];
-  int E;
+// A wave's state: 16 query rows, this lane's being number lane & 15.  KS = steps of 64 dimensions.
+template <int KS>
+struct AttnRows {
+  i4 q[3][KS];   // query digits, lowest first
+  int qe;        // their power of two
+  float qn;      // 1, or NaN for a query that is not finite
+  int seen;      // keys that the row sees
+  float M, sum;  // running maximum, sum of weights
+  f4 o[4 * KS];  // sums over the values: dimensions 16 d + 4 (lane >> 4) .. + 3
+  int E;         // largest value exponent
 };
 
-template <int KS, int QT>
-TL_DEVICE void attn_begin(AttnWave<KS, QT>& s, const Q8AttnArgs& a, int b, int h, int r0, int rows, long long pos) {
-  const int lane = threadIdx.x & 63, kg = lane >> 4;
+TL_DEVICE void attn_load_q(const Q8AttnArgs& a, const float* src, bool in, int d, float (&x)[16]) {
+  if (a.vec) {
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = r0 + 16 * t + (lane & 15);
-    const bool in = r < rows;
-    const int i = in ? r / a.mul : 0;
-    const long long p = pos + i;
-    s.seen[t] = in && p >= 0 && p < a.l.seq_len ? (int)p + 1 : 0;
-    const float* src = a.q + ((long long)b * a.call.n_tokens + i) * a.q_stride +
-                       (long long)(h * a.mul + (in ? r - i * a.mul : 0)) * a.l.head_size;
-    float x[KS][16];
-    unsigned top = 0;
+    for (int e = 0; e < 16; e += 4) {
+      f4 v = {0.f, 0.f, 0.f, 0.f};
+      if (in && d + e < a.l.head_size) v = *reinterpret_cast<const f4*>(src + d + e);
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int d = 64 * k + 16 * kg;
-      if (a.vec) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          f4 v = {0.f, 0.f, 0.f, 0.f};
-          if (in && d + e < a.l.head_size) v = *reinterpret_cast<const f4*>(src + d + e);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) x[k][e + c] = v[c];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[k][e] = in && d + e < a.l.head_size ? src[d + e] : 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
+      for (int c = 0; c < 4; ++c) x[e + c] = v[c];
     }
-    top = rows_umax(top);
-    s.qn[t] = top < 0x7f800000u ? 1.f : __builtin_nanf("");
-    s.qe[t] = top < 0x7f800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
+  } else {
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        unsigned n[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          n[c] = (unsigned)(int)rintf(__builtin_ldexpf(x[k][4 * e + c], -s.qe[t]) * kDigits);
-        int p0, p1, p2;
-        digits4(n, p0, p1, p2);
-        s.q[t][0][k][e] = p0;
-        s.q[t][1][k][e] = p1;
-        s.q[t][2][k][e] = p2;
-      }
-    s.M[t] = kNone;
-    s.sum[t] = 0.f;
-#pragma unroll
-    for (int d = 0; d < 4 * KS; ++d) s.o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < 16; ++e) x[e] = in && d + e < a.l.head_size ? src[d + e] : 0.f;
   }
+}
+
+// Rows r0 .. r0 + 15 of the `rows` of (b, h).  A row behind the last sees what the tile sees and is never stored.
+template <int KS>
+TL_DEVICE void attn_begin(AttnRows<KS>& s, const Q8AttnArgs& a, int b, int h, int r0, int rows, long long pos, int T) {
+  const int lane = threadIdx.x & 63, kg = lane >> 4;
+  const int r = r0 + (lane & 15);
+  const bool in = r < rows;
+  const int i = in ? r / a.mul : 0;
+  const long long p = pos + i;
+  s.seen = !in ? T : p >= 0 && p < a.l.seq_len ? (int)p + 1 : 0;
+  const float* src = a.q + ((long long)b * a.call.n_tokens + i) * a.q_stride +
+                     (long long)(h * a.mul + (in ? r - i * a.mul : 0)) * a.l.head_size;
+  float x[KS][16];
+  unsigned top = 0;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) attn_load_q(a, src, in, 64 * k + 16 * kg, x[k]);
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
+  top = rows_umax(top);
+  s.qn = top < 0x7f800000u ? 1.f : __builtin_nanf("");
+  s.qe = top < 0x7f800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      unsigned n[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) n[c] = (unsigned)(int)rintf(__builtin_ldexpf(x[k][4 * e + c], -s.qe) * kDigits);
+      int p0, p1, p2;
+      digits4(n, p0, p1, p2);
+      s.q[0][k][e] = p0;
+      s.q[1][k][e] = p1;
+      s.q[2][k][e] = p2;
+    }
+  s.M = kNone;
+  s.sum = 0.f;
+#pragma unroll
+  for (int d = 0; d < 4 * KS; ++d) s.o[d] = f4{0.f, 0.f, 0.f, 0.f};
   s.E = -126;
 }
 
-// NT tiles of 64 keys from t0 on.
-template <int KS, int QT, int NT>
-TL_DEVICE void attn_keys(AttnWave<KS, QT>& s, const Q8AttnArgs& a, const int8_t* k, const int8_t* v, const float* ks,
-                         const float* vs, int t0, int T) {
-  constexpr int DT = 4 * KS;
-  const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4;
-  const int lanes = a.l.lanes;
-
-  // scales of this lane's sixteen keys in each tile; those of keys that nobody sees are 0
+// Scales of this lane's sixteen keys in each of NT tiles of 64 from t0 on; those of keys that nobody sees are 0.
+template <int NT>
+struct AttnScales {
   float sk[NT], f[NT], lift[NT];
   int e[NT];
+  TL_DEVICE void load(const Q8AttnArgs& a, const float* ks, const float* vs, int t0, int T) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int t = t0 + 64 * n + 16 * g;
+      const int j = min(t, T - 1) >> a.l.block_log2;
+      sk[n] = t < T ? ks[j] : 0.f;
+      f[n] = t < T ? vs[j] : 0.f;
+    }
+  }
+};
+
+// One step of NT tiles of 64 keys from t0 on.  Key: (tile, 16-key step, 64-dimension step), Val: (tile, 16-dimension
+// step) -> sixteen codes.  ready() runs between the two products.
+template <int KS, int NT, class Key, class Val, class Ready>
+TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
+  constexpr int DT = 4 * KS;
+  const int g = (threadIdx.x & 63) >> 4;
   int top = s.E;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int t = t0 + 64 * n + 16 * g;
-    const bool in = t < T;
-    const int j = min(t, T - 1) >> a.l.block_log2;
-    sk[n] = in ? ks[j] : 0.f;
-    f[n] = in ? vs[j] : 0.f;
-    e[n] = f[n] > 0.f ? __builtin_amdgcn_frexp_expf(f[n]) : -126;
-    top = max(top, e[n]);
+    c.e[n] = c.f[n] > 0.f ? __builtin_amdgcn_frexp_expf(c.f[n]) : -126;
+    top = max(top, c.e[n]);
   }
   {
     v2u r = __builtin_amdgcn_permlane32_swap((unsigned)top, (unsigned)top, false, false);
@@ -182,112 +188,154 @@ TL_DEVICE void attn_keys(AttnWave<KS, QT>& s, const Q8AttnArgs& a, const int8_t*
   s.E = top;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    e[n] = max(e[n], top - 40);
-    lift[n] = f[n] == f[n] ? __builtin_ldexpf(1.f, top - e[n]) : f[n];  // a NaN scale makes the sum NaN
-    f[n] = __builtin_ldexpf(f[n], -e[n]) * kDigits;
+    c.e[n] = max(c.e[n], top - 40);
+    c.lift[n] = c.f[n] == c.f[n] ? __builtin_ldexpf(1.f, top - c.e[n]) : c.f[n];  // a NaN scale makes the sum NaN
+    c.f[n] = __builtin_ldexpf(c.f[n], -c.e[n]) * kDigits;
   }
 
-  // scores
-  i4 p[QT][NT][3];
-  float alpha[QT];
-  f4 x[QT][NT][4];
+  // Scores.  Each turn asks for the next one's operands, starts this one's products and finishes the last one's, so
+  // that neither LDS nor the matrix pipe is waited for.
+  f4 x[NT][4];
+  {
+    i4 k[2][KS], acc[2][3];
+    float c1 = 0.f, ce = 0.f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float c1[QT];
+    for (int d = 0; d < KS; ++d) k[0][d] = key(0, 0, d);
 #pragma unroll
-    for (int t = 0; t < QT; ++t) c1[t] = __builtin_ldexpf(a.c0 * sk[n], s.qe[t]) * s.qn[t];
+    for (int u = 0; u <= 4 * NT; ++u) {
+      if (u + 1 < 4 * NT) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int8_t* kp = k + (long long)(t0 + 64 * n + 16 * (row >> 2) + 4 * j + (row & 3)) * lanes;
-      i4 key[KS];
-#pragma unroll
-      for (int c = 0; c < KS; ++c) {
-        const int d = 64 * c + 16 * g;
-        key[c] = *reinterpret_cast<const i4*>(kp + (d < lanes ? d : 0));  // the query's digits are 0 from lanes on
+        for (int d = 0; d < KS; ++d) k[(u + 1) & 1][d] = key((u + 1) / 4, (u + 1) & 3, d);
       }
+      if (u < 4 * NT) {
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        i4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+        for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(k[u & 1][0], s.q[z][0], i4{0, 0, 0, 0});
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          hi = mfma(key[c], s.q[t][2][c], hi);
-          lo = mfma(key[c], s.q[t][1][c], lo);
+        for (int d = 1; d < KS; ++d)
+#pragma unroll
+          for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(k[u & 1][d], s.q[z][d], acc[u & 1][z]);
+      }
+      if (u > 0) {
+        const int n = (u - 1) / 4, j = (u - 1) & 3;
+        if (j == 0) {
+          c1 = __builtin_ldexpf(a.c0 * c.sk[n], s.qe) * s.qn;
+          ce = (float)c.e[n];
         }
-        lo <<= 8;
-#pragma unroll
-        for (int c = 0; c < KS; ++c) lo = mfma(key[c], s.q[t][0][c], lo);
+        const i4(&r)[3] = acc[(u - 1) & 1];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          x[t][n][j][i] = fmaf((float)hi[i], 65536.f * c1[t], fmaf((float)lo[i], c1[t], (float)e[n]));
+          x[n][j][i] = fmaf((float)r[2][i], 65536.f * c1, fmaf((float)((r[1][i] << 8) + r[0][i]), c1, ce));
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
-  // weights
+  const int left = s.seen - t0 - 16 * g;  // keys of this lane's first tile and behind it that the row sees
+  if (edge) {
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    float m = kNone;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int first = t0 + 64 * n + 16 * g;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (first + 4 * j + i >= s.seen[t]) x[t][n][j][i] = -INFINITY;
-          m = fmaxf(m, x[t][n][j][i]);
-        }
-    }
-    m = fmaxf(rows_max(m), s.M[t]);
-    alpha[t] = __builtin_amdgcn_exp2f(s.M[t] - m);
-    s.M[t] = m;
-    float sum = 0.f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int first = t0 + 64 * n + 16 * g;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        unsigned w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = __builtin_amdgcn_exp2f(x[t][n][j][i] - m);
-          sum = first + 4 * j + i >= s.seen[t] ? sum : fmaf(u, lift[n], sum);  // 0 x NaN of a block behind the row
-          w[i] = __float_as_uint(fmaf(u, f[n], 8388608.f));  // its low bytes: the nearest integer
-        }
-        int p0, p1, p2;
-        digits4(w, p0, p1, p2);
-        p[t][n][0][j] = p0;
-        p[t][n][1][j] = p1;
-        p[t][n][2][j] = p2;
-      }
-    }
-    s.sum[t] = fmaf(__builtin_ldexpf(s.sum[t], grow), alpha[t], sum);
+        for (int i = 0; i < 4; ++i)
+          if (64 * n + 4 * j + i >= left) x[n][j][i] = -INFINITY;
   }
+  float m = s.M;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = fmaxf(m, x[n][j][i]);
+  m = rows_max(m);
+  const float alpha = __builtin_amdgcn_exp2f(s.M - m);
+  s.M = m;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][j][i] = __builtin_amdgcn_exp2f(x[n][j][i] - m);
+  float sum = 0.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float part = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part += (x[n][j][0] + x[n][j][1]) + (x[n][j][2] + x[n][j][3]);
+    if (edge && 64 * n >= left) continue;  // 0 x NaN of a block behind the row
+    sum = fmaf(part, c.lift[n], sum);
+  }
+  s.sum = fmaf(__builtin_ldexpf(s.sum, grow), alpha, sum);
+  i4 p[NT][3];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unsigned w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmaf(x[n][j][i], c.f[n], 8388608.f));  // low bytes: the nearest integer
+      int p0, p1, p2;
+      digits4(w, p0, p1, p2);
+      p[n][0][j] = p0;
+      p[n][1][j] = p1;
+      p[n][2][j] = p2;
+    }
 
-  // values
-  const int8_t* vp = v + (long long)((t0 >> 4) + g) * (16 * lanes) + 16 * row;
+  ready();
+  // values, in the same turns
+  {
+    i4 v[2][NT], acc[2][3];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) {
-    if (16 * d >= lanes) continue;
-    i4 val[NT];
+    for (int n = 0; n < NT; ++n) v[0][n] = val(n, 0);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) val[n] = *reinterpret_cast<const i4*>(vp + (long long)(64 * n) * lanes + 256 * d);
+    for (int u = 0; u <= DT; ++u) {
+      if (u + 1 < DT) {
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      i4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        hi = mfma(val[n], p[t][n][2], hi);
-        lo = mfma(val[n], p[t][n][1], lo);
+        for (int n = 0; n < NT; ++n) v[(u + 1) & 1][n] = val(n, u + 1);
       }
-      lo <<= 8;
+      if (u < DT) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) lo = mfma(val[n], p[t][n][0], lo);
+        for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(v[u & 1][0], p[0][z], i4{0, 0, 0, 0});
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s.o[t][d][i] = fmaf(s.o[t][d][i], alpha[t], fmaf((float)hi[i], 65536.f, (float)lo[i]));
+        for (int n = 1; n < NT; ++n)
+#pragma unroll
+          for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(v[u & 1][n], p[n][z], acc[u & 1][z]);
+      }
+      if (u > 0) {
+        const i4(&r)[3] = acc[(u - 1) & 1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s.o[u - 1][i] = fmaf(s.o[u - 1][i], alpha, fmaf((float)r[2][i], 65536.f, (float)((r[1][i] << 8) + r[0][i])));
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+}
+
+// The least number of keys that one of the wave's rows sees.
+TL_DEVICE int attn_least(int seen) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) seen = min(seen, __shfl_xor(seen, o, 64));
+  return __builtin_amdgcn_readfirstlane(seen);
+}
+
+struct AttnUnit {  // what a workgroup works on
+  int b, h, r0, rows, nr, T;
+  long long pos;
+};
+// Row tile `tile` of R rows of pair (b, h); false if the sequence has no such rows.
+TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, AttnUnit& w) {
+  w.h = pair % a.l.heads;
+  w.b = pair / a.l.heads;
+  const int count = a.call.n_d ? min(max(a.call.n_d[w.b], 0), a.call.n_tokens) : a.call.n_tokens;
+  w.pos = a.call.pos_d[w.b];
+  w.rows = count * a.mul;
+  w.r0 = tile * R;
+  if (w.r0 >= w.rows) return false;
+  w.nr = min(R, w.rows - w.r0);
+  const long long first = w.pos + w.r0 / a.mul, last = w.pos + (w.r0 + w.nr - 1) / a.mul;
+  w.T = first >= a.l.seq_len ? 0 : (int)max(0LL, min(last + 1, (long long)a.l.seq_len));
+  return true;
 }
 
 // What a wave, a workgroup or a split knows of a row: sum_t 2^(x_t) v_t = 2^M o and sum_t 2^(x_t) = 2^(M - E) sum.
@@ -299,85 +347,111 @@ TL_DEVICE void row_join(float M, float E, const RowPart& r, float& wo, float& ws
   ws = r.sum == 0.f ? 0.f : __builtin_amdgcn_exp2f((r.M - M) + (E - r.E)) * r.sum;
 }
 
-// One workgroup: QT tiles of 16 query rows of one (sequence, K/V head), and of their keys the share of split
-// blockIdx's low part; its waves take runs of 64-key tiles.
-template <int KS, int QT>
-__global__ void __launch_bounds__(256) k_q8_attn(Q8AttnArgs a) {
+// Dimensions d .. d + 3 of row r of the unit, from its sums.  A row without keys is zeros.
+TL_DEVICE void attn_store(const Q8AttnArgs& a, const AttnUnit& w, int r, int d, f4 o, float M, float sum, float E) {
+  const int hs = a.l.head_size, i = (w.r0 + r) / a.mul;
+  float* dst = a.out + ((long long)w.b * a.call.n_tokens + i) * a.out_stride + (long long)(w.h * a.mul + w.r0 + r - i * a.mul) * hs + d;
+  const float inv = 1.f / (sum * kDigits);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = M == kNone && sum == 0.f ? 0.f : __builtin_ldexpf(o[e] * inv, (int)E);
+  if (a.vec) {
+    *reinterpret_cast<f4*>(dst) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < hs) dst[e] = o[e];
+  }
+}
+
+// 16 bytes a lane from memory to LDS, at `to` + 16 * lane; lds_wait: everybody's have arrived.  Written out, because
+// with the builtin the compiler waits for every load under way before the next read of any LDS.  m0 has no other use
+// in a kernel that calls this.
+TL_DEVICE void lds_bring(const int8_t* from, i4* to) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)to);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+}
+TL_DEVICE void lds_wait() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
+
+// Few rows: one workgroup takes 16 query rows of one (sequence, K/V head) and, of their keys, every nsplit-th run of
+// a 64-key tile for each of its waves; the waves' results are joined in LDS, the workgroups' by k_q8_attn_join.
+template <int KS>
+__global__ void __launch_bounds__(KS < 4 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const Q8KVLayer& l = a.l;
-  constexpr int R = 16 * QT;
   unsigned u = blockIdx.x;
   const int split = u % a.nsplit;
-  u /= a.nsplit;
-  const unsigned unit = u;
-  const unsigned pairs = a.call.n_batches * l.heads;
-  const int tile = a.tiles - 1 - u / pairs;  // the longest rows first
-  u %= pairs;
-  const int h = u % l.heads, b = u / l.heads;
-  const int count = a.call.n_d ? min(max(a.call.n_d[b], 0), a.call.n_tokens) : a.call.n_tokens;
-  const int rows = count * a.mul, r0 = tile * R;
-  if (r0 >= rows) return;
-  const long long pos = a.call.pos_d[b];
-  const int nr = min(R, rows - r0);
-  const int T = pos + r0 / a.mul >= l.seq_len ? 0 : (int)max(0LL, min(pos + (r0 + nr - 1) / a.mul + 1, (long long)l.seq_len));
+  const unsigned unit = u / a.nsplit, pairs = a.call.n_batches * l.heads;
+  AttnUnit w;
+  if (!attn_unit(a, unit % pairs, a.tiles - 1 - unit / pairs, 16, w)) return;
 
-  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-  const int tiles = (T + 63) / 64, share = (tiles + a.nsplit - 1) / a.nsplit;
-  const int lo = min(tiles, split * share), hi = min(tiles, lo + share);
-  const int each = (hi - lo + waves - 1) / waves;
-  const int from = __builtin_amdgcn_readfirstlane(min(hi, lo + wave * each));
-  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + each));
-
-  AttnWave<KS, QT> s;
-  attn_begin<KS, QT>(s, a, b, h, r0, rows, pos);
-  const int8_t* k = l.k + b * l.seq_codes + h * l.head_codes;
-  const int8_t* v = l.v + b * l.seq_codes + h * l.head_codes;
-  const float* ks = l.ks + b * l.seq_scales + h * l.head_scales;
-  const float* vs = l.vs + b * l.seq_scales + h * l.head_scales;
-  int at = from;
-  for (; at + 2 <= to; at += 2) attn_keys<KS, QT, 2>(s, a, k, v, ks, vs, 64 * at, T);
-  if (at < to) attn_keys<KS, QT, 1>(s, a, k, v, ks, vs, 64 * at, T);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  AttnRows<KS> s;
+  attn_begin<KS>(s, a, w.b, w.h, w.r0, w.rows, w.pos, w.T);
+  const int least = attn_least(s.seen);
+  const int8_t* k = l.k + w.b * l.seq_codes + w.h * l.head_codes;
+  const int8_t* v = l.v + w.b * l.seq_codes + w.h * l.head_codes;
+  const float* ks = l.ks + w.b * l.seq_scales + w.h * l.head_scales;
+  const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
+  const int row = lane & 15, g = lane >> 4;
+  for (int t0 = 64 * (split * waves + wave); t0 < w.T; t0 += 64 * waves * a.nsplit) {
+    const int8_t* kp = k + (long long)(t0 + 16 * (row >> 2) + (row & 3)) * l.lanes;
+    const int8_t* vp = v + (long long)((t0 >> 4) + g) * (16 * l.lanes) + 16 * row;
+    i4 kc[4][KS], vc[4 * KS];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < KS; ++c) {
+        const int d = 64 * c + 16 * g;
+        kc[j][c] = *reinterpret_cast<const i4*>(kp + 4 * j * l.lanes + (d < l.lanes ? d : 0));  // the query's digits are 0 from lanes on
+      }
+    AttnScales<1> sc;
+    sc.load(a, ks, vs, t0, w.T);
+#pragma unroll
+    for (int d = 0; d < 4 * KS; ++d)
+      vc[d] = *reinterpret_cast<const i4*>(vp + (16 * d < l.lanes ? 256 * d : 0));
+    attn_step<KS, 1>(s, a, sc, t0, t0 + 64 > least, [&](int, int j, int c) { return kc[j][c]; }, [&](int, int d) { return vc[d]; }, [] {});
+  }
 
   // join the waves' rows
   const int hs = l.head_size, step = 64 * KS + 4;
   float* stat = lds + waves * a.lrows * step;
+  s.sum = rows_sum(s.sum);
+  if (row < w.nr) {
+    float* dst = lds + (wave * a.lrows + row) * step + 4 * g;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = 16 * t + (lane & 15);
-    s.sum[t] = rows_sum(s.sum[t]);
-    if (r >= nr) continue;
-    float* dst = lds + (wave * a.lrows + r) * step + 4 * (lane >> 4);
-#pragma unroll
-    for (int d = 0; d < 4 * KS; ++d) *reinterpret_cast<f4*>(dst + 16 * d) = s.o[t][d];
+    for (int d = 0; d < 4 * KS; ++d) *reinterpret_cast<f4*>(dst + 16 * d) = s.o[d];
     if (lane < 16) {
-      stat[3 * (wave * a.lrows + r)] = s.M[t];
-      stat[3 * (wave * a.lrows + r) + 1] = s.sum[t];
-      stat[3 * (wave * a.lrows + r) + 2] = (float)s.E;
+      stat[3 * (wave * a.lrows + row)] = s.M;
+      stat[3 * (wave * a.lrows + row) + 1] = s.sum;
+      stat[3 * (wave * a.lrows + row) + 2] = (float)s.E;
     }
   }
   __syncthreads();
   const int quads = (hs + 3) / 4;
-  for (int it = threadIdx.x; it < nr * quads; it += blockDim.x) {
+  for (int it = threadIdx.x; it < w.nr * quads; it += blockDim.x) {
     const int r = it / quads, d = (it - r * quads) * 4;
     float M = kNone, E = -126.f;
-    for (int w = 0; w < waves; ++w) {
-      M = fmaxf(M, stat[3 * (w * a.lrows + r)]);
-      E = fmaxf(E, stat[3 * (w * a.lrows + r) + 2]);
+    for (int n = 0; n < waves; ++n) {
+      M = fmaxf(M, stat[3 * (n * a.lrows + r)]);
+      E = fmaxf(E, stat[3 * (n * a.lrows + r) + 2]);
     }
     f4 o = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
-    for (int w = 0; w < waves; ++w) {
-      const float* st = stat + 3 * (w * a.lrows + r);
+    for (int n = 0; n < waves; ++n) {
+      const float* st = stat + 3 * (n * a.lrows + r);
       float wo, ws;
       row_join(M, E, {st[0], st[1], st[2]}, wo, ws);
-      const f4 x = *reinterpret_cast<const f4*>(lds + (w * a.lrows + r) * step + d);
+      const f4 x = *reinterpret_cast<const f4*>(lds + (n * a.lrows + r) * step + d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], wo, o[e]);
       sum += ws;
     }
     if (a.nsplit > 1) {
-      float* dst = a.part + (((long long)unit * a.nsplit + split) * R + r) * (hs + 4);
+      float* dst = a.part + (((long long)unit * a.nsplit + split) * 16 + r) * (hs + 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (d + e < hs) dst[d + e] = o[e];
@@ -386,21 +460,79 @@ __global__ void __launch_bounds__(256) k_q8_attn(Q8AttnArgs a) {
         dst[hs + 1] = sum;
         dst[hs + 2] = E;
       }
-      continue;
-    }
-    const int i = (r0 + r) / a.mul;
-    float* dst = a.out + ((long long)b * a.call.n_tokens + i) * a.out_stride + (long long)(h * a.mul + r0 + r - i * a.mul) * hs + d;
-    const float inv = 1.f / (sum * kDigits);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = M == kNone && sum == 0.f ? 0.f : __builtin_ldexpf(o[e] * inv, (int)E);
-    if (a.vec) {
-      *reinterpret_cast<f4*>(dst) = o;
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (d + e < hs) dst[e] = o[e];
+      attn_store(a, w, r, d, o, M, sum, E);
     }
   }
+}
+
+// Many rows: each of four waves takes 16 query rows of one (sequence, K/V head), and all of them the same keys, which
+// pass through LDS in chunks of NT tiles: the values' codes come in while the scores are computed, the next
+// chunk's keys while the values are.  LDS holds the codes in the order in which the lanes want them, one KiB for
+// each operand of a product, so that a load (16 bytes a lane, memory to LDS) and a read are both linear in the lane.
+template <int KS, int NT>
+__global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs a) {
+  keep_implicit_args();  // common.hpp
+  __shared__ __attribute__((aligned(1024))) i4 kbuf[NT * 4 * KS * 64];
+  __shared__ __attribute__((aligned(1024))) i4 vbuf[NT * 4 * KS * 64];
+  const Q8KVLayer& l = a.l;
+  const unsigned pairs = a.call.n_batches * l.heads;
+  AttnUnit w;
+  if (!attn_unit(a, blockIdx.x % pairs, a.tiles - 1 - blockIdx.x / pairs, 64, w)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = lane & 15, g = lane >> 4;
+  const int8_t* k = l.k + w.b * l.seq_codes + w.h * l.head_codes;
+  const int8_t* v = l.v + w.b * l.seq_codes + w.h * l.head_codes;
+  const float* ks = l.ks + w.b * l.seq_scales + w.h * l.head_scales;
+  const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
+
+  // wave i brings operands i, i + 4, ...; tiles behind the last key are not brought
+  auto keys_in = [&](int t0) {
+#pragma unroll
+    for (int f = 0; f < NT * KS; ++f) {
+      const int n = f / KS, c = f % KS, j = wave;  // operand (n, j, c)
+      if (t0 + 64 * n >= w.T) continue;
+      const int d = 64 * c + 16 * g;
+      const int8_t* src = k + (long long)(t0 + 64 * n + 16 * (row >> 2) + 4 * j + (row & 3)) * l.lanes + (d < l.lanes ? d : 0);
+      lds_bring(src, &kbuf[((n * 4 + j) * KS + c) * 64]);
+    }
+  };
+  auto values_in = [&](int t0) {
+#pragma unroll
+    for (int f = 0; f < NT * KS; ++f) {
+      const int n = f / KS, d = (f % KS) * 4 + wave;  // operand (n, d)
+      if (t0 + 64 * n >= w.T || 16 * d >= l.lanes) continue;
+      const int8_t* src = v + (long long)((t0 >> 4) + 4 * n + g) * (16 * l.lanes) + 256 * d + 16 * row;
+      lds_bring(src, &vbuf[(n * 4 * KS + d) * 64]);
+    }
+  };
+
+  if (w.T > 0) keys_in(0);
+  AttnRows<KS> s;
+  attn_begin<KS>(s, a, w.b, w.h, w.r0 + 16 * wave, w.rows, w.pos, w.T);
+  const int least = attn_least(s.seen);
+  const int most = -attn_least(-s.seen);
+  for (int t0 = 0; t0 < w.T; t0 += 64 * NT) {
+    AttnScales<NT> sc;
+    sc.load(a, ks, vs, t0, w.T);
+    lds_wait();  // this chunk's keys are in, and every wave has left the last chunk's values
+    values_in(t0);
+    auto ready = [&] {
+      lds_wait();  // the values are in, and every wave has left this chunk's keys
+      if (t0 + 64 * NT < w.T) keys_in(t0 + 64 * NT);
+    };
+    if (t0 >= most) {  // the other waves' rows see further
+      ready();
+      continue;
+    }
+    attn_step<KS, NT>(s, a, sc, t0, t0 + 64 * NT > least, [&](int n, int j, int c) { return kbuf[((n * 4 + j) * KS + c) * 64 + lane]; },
+                      [&](int n, int d) { return vbuf[(n * 4 * KS + d) * 64 + lane]; }, ready);
+  }
+  s.sum = rows_sum(s.sum);
+  if (16 * wave + row < w.nr)
+#pragma unroll
+    for (int d = 0; d < 4 * KS; ++d)
+      if (16 * d + 4 * g < l.head_size) attn_store(a, w, 16 * wave + row, 16 * d + 4 * g, s.o[d], s.M, s.sum, (float)s.E);
 }
 
 // Joins the splits of one (row tile, row): one wave each, lanes along the dimensions.
@@ -439,29 +571,35 @@ constexpr int kAttnBlocks = 512;  // workgroups that keep the card's 256 CUs bus
 
 // How a call's rows and keys are divided.
 struct AttnPlan {
-  int qt, waves, nsplit;
+  bool many;
+  int waves, nsplit;
   long long tiles, units;
 };
 static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads) {
   AttnPlan p;
   const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads), pairs = (long long)n_batches * c->n_kv_heads;
-  p.qt = rows > 16 && c->head_size <= 128 && pairs * ((rows + 31) / 32) >= kAttnBlocks ? 2 : 1;
-  p.tiles = (rows + 16 * p.qt - 1) / (16 * p.qt);
+  p.many = pairs * ((rows + 63) / 64) >= kAttnBlocks / 2 && rows >= 64;
+  p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
-  p.waves = 4;
+  p.waves = p.many || c->head_size > 192 ? 4 : 8;
   const long long most = (c->seq_len + 64LL * p.waves - 1) / (64 * p.waves);  // every wave has a tile to do
-  p.nsplit = (int)max(1LL, min(most, min(64LL, kAttnBlocks / p.units)));
+  p.nsplit = p.many ? 1 : (int)max(1LL, min(most, min(64LL, kAttnBlocks / p.units)));
   return p;
 }
 
-template <int KS, int QT>
+template <int KS>
 static hipError_t attn_launch(const Q8AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+  const dim3 grid((unsigned)(p.units * p.nsplit)), block(64 * p.waves);
+  if (p.many) {
+    hipLaunchKernelGGL((k_q8_attn_many<KS, KS <= 2 ? 4 : 2>), grid, block, 0, s, a);
+    return hipGetLastError();
+  }
   const size_t lds = (size_t)p.waves * a.lrows * (64 * KS + 4 + 3) * sizeof(float);
   if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)k_q8_attn<KS, QT>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    const hipError_t e = hipFuncSetAttribute((const void*)k_q8_attn_few<KS>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((k_q8_attn<KS, QT>), dim3((unsigned)(p.units * p.nsplit)), dim3(64 * p.waves), lds, s, a);
+  hipLaunchKernelGGL((k_q8_attn_few<KS>), grid, block, lds, s, a);
   return hipGetLastError();
 }
 
@@ -496,7 +634,7 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   const int mul = n_heads / c->n_kv_heads;
   const tl::AttnPlan p = tl::attn_plan(c, n_batches, n_tokens, n_heads);
   if ((long long)n_tokens * mul > 0x7fffffffLL - 64 || p.units * p.nsplit > 0x7fffffffLL / 16) return THABLAS_STATUS_NOT_SUPPORTED;
-  const size_t need = p.nsplit > 1 ? (size_t)p.units * p.nsplit * 16 * p.qt * (c->head_size + 4) * sizeof(float) : 0;
+  const size_t need = p.nsplit > 1 ? (size_t)p.units * p.nsplit * 16 * (c->head_size + 4) * sizeof(float) : 0;
   if (need && (!work || ((uintptr_t)work & 15) || work_bytes < need)) return THABLAS_STATUS_INVALID_VALUE;
   a.call = {pos_d, n_d, n_batches, n_tokens};
   a.q = q;
@@ -508,7 +646,7 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   a.mul = mul;
   a.tiles = (int)p.tiles;
   a.nsplit = p.nsplit;
-  a.lrows = (int)min((long long)n_tokens * mul, 16LL * p.qt);
+  a.lrows = (int)min((long long)n_tokens * mul, 16LL);
   a.vec = tl::q8kv_vec4(c->head_size, q_stride, q, out) && out_stride % 4 == 0;
   a.c0 = (float)(1.4426950408889634 / __builtin_sqrt((double)c->head_size) / tl::kDigits);
   tl::Q8KVDevice dev(handle->current_gpu_id);
@@ -516,11 +654,12 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   const int ks = (a.l.lanes + 63) / 64;
   hipStream_t s = handle->calc_stream;
   hipError_t e;
-  if (ks == 1) e = p.qt == 2 ? tl::attn_launch<1, 2>(a, p, s) : tl::attn_launch<1, 1>(a, p, s);
-  else if (ks == 2) e = p.qt == 2 ? tl::attn_launch<2, 2>(a, p, s) : tl::attn_launch<2, 1>(a, p, s);
-  else e = ks == 3 ? tl::attn_launch<3, 1>(a, p, s) : tl::attn_launch<4, 1>(a, p, s);
+  if (ks == 1) e = tl::attn_launch<1>(a, p, s);
+  else if (ks == 2) e = tl::attn_launch<2>(a, p, s);
+  else if (ks == 3) e = tl::attn_launch<3>(a, p, s);
+  else e = tl::attn_launch<4>(a, p, s);
   if (e != hipSuccess) return THABLAS_STATUS_EXECUTION_FAILED;
   if (p.nsplit > 1)
-    hipLaunchKernelGGL(tl::k_q8_attn_join, dim3((unsigned)(p.units * 16 * p.qt)), dim3(64), 0, s, a, 16 * p.qt);
+    hipLaunchKernelGGL(tl::k_q8_attn_join, dim3((unsigned)(p.units * 16)), dim3(64), 0, s, a, 16);
   return tl::q8kv_status(hipGetLastError());
 }

@@ -83,9 +83,9 @@ class Cache:
         scale = np.repeat(self.scales[w][:, layer], self.block, axis=-1)[..., None].astype(dtype)
         return self.codes[w][:, layer, :, :, :self.hs].astype(dtype) * scale
 
-    def attend(self, layer, pos, n, n_tokens, q, mul):
+    def attend(self, layer, pos, n, n_tokens, q, mul, some=None):
         """q [B, n_tokens, H * mul, hs] -> (out in 64 bits, bound of an fp32-accurate result's error), rows that are
-        not computed NaN.
+        not computed (or not among `some`) NaN.
 
         The bound, with u = 2^-24 and T keys in sight: a score is off by at most E = u (hs sum |q||k| + 2 max|q|
         sum |k|) / sqrt(hs) (a sum of hs rounded products, or a query held in 24 bits of its largest component) and
@@ -99,6 +99,8 @@ class Cache:
         for b in range(len(pos)):
             for i in range(min(max(n[b], 0), n_tokens)):
                 p = pos[b] + i
+                if some is not None and i not in some:
+                    continue
                 if p < 0 or p >= self.S:
                     out[b, i] = 0
                     continue

@@ -239,6 +239,15 @@ ATTENDS = [  # B, L, H, mul, hs, S, block, pos, n, n_tokens, pad, shift
     (2, 1, 2, 1, 32, 90, 16, [-1, 90], None, 1, 0, 0),
     (2, 1, 2, 2, 32, 90, 16, [2147483647, -2147483648], None, 3, 0, 0),
     (2, 1, 2, 1, 32, 90, 16, [4, 5], [-1, 99], 6, 0, 0),
+] + [  # rows enough to fill the card: a few hundred tiles of 64
+    (16, 1, 16, 1, 64, 200, 32, [7 * b for b in range(16)], [66 - 4 * b for b in range(16)], 66, 0, 0),
+    (32, 2, 4, 3, 48, 700, 16, [20 * b for b in range(32)], None, 30, 0, 0),
+    (64, 1, 2, 8, 128, 300, 64, [4 * b for b in range(64)], [b % 18 for b in range(64)], 17, 0, 0),
+    (32, 1, 8, 5, 130, 350, 128, [9 * b for b in range(32)], None, 13, 2, 1),
+    (64, 1, 4, 1, 200, 330, 32, [260, 3] * 32, [70, 65] * 32, 70, 4, 4),
+    (64, 1, 4, 1, 256, 70, 16, [0, -5, 69, 70] * 16, None, 65, 0, 0),
+    (64, 1, 4, 2, 8, 90, 64, [80, -40, -100, 2147483647] * 16, None, 33, 0, 0),
+    (1, 1, 2, 2, 128, 4300, 64, [100], None, 4160, 0, 0),
 ]
 
 
@@ -260,11 +269,14 @@ def test_attention(gpu, handle, case):
     counts = [nt] * B if n is None else n
     upto = [min(max(p + c, 0), S) for p, c in zip(pos, counts)]
     ref, dev = filled(gpu, handle, r, B, L, H, hs, S, block, upto, layer)
+    some = range(nt) if nt < 1000 else sorted({0, 1, nt - 1, *r.integers(0, nt, 40).tolist()})
     q = (r.standard_normal((B, nt, H * mul, hs)) * r.uniform(0.2, 3, (B, nt, H * mul, 1))).astype(np.float32)
     got = dev.attend(layer, pos, n, q, pad, shift)
-    want, bound = ref.attend(layer, pos, counts, nt, q, mul)
+    want, bound = ref.attend(layer, pos, counts, nt, q, mul, some)
     assert (got[:, :, H * mul * hs:] == -77).all(), "written behind a row's end"
-    hold(got[:, :, :H * mul * hs].reshape(want.shape), want, bound, "attention")
+    hold(got[:, some, :H * mul * hs].reshape(want[:, some].shape), want[:, some], bound[:, some], "attention")
+    for b in range(B):
+        assert np.isfinite(got[b, :max(counts[b], 0), :H * mul * hs]).all() and (got[b, max(counts[b], 0):] == -77).all()
     dev.check("attention leaves the cache")
 
 
