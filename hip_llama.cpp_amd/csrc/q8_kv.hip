@@ -39,10 +39,12 @@ extern "C" int thallama_q8_kv_map(Q8KVCache* c, void* mem, int n_batches, int n_
 
 namespace tl {
 
-// Dimensions d .. d + 3 of a row; those from head_size on read as 0.
+// Dimensions d .. d + 3 of a row; those from head_size on read as 0.  A call passes over its rows once: nontemporal, which
+// is what carries the large calls (8 x 2048 rows of 4096 and their codes, MI355X: stored in 157 us without, 120 with, read
+// back in 134 and 129; one row each of sixteen sequences' blocks read back in 8.2 and 6.2).
 template <bool VEC>
 TL_DEVICE f4 row4_load(const float* row, int d, int head_size) {
-  if constexpr (VEC) return *reinterpret_cast<const f4*>(row + d);
+  if constexpr (VEC) return __builtin_nontemporal_load(reinterpret_cast<const f4*>(row + d));
   f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -52,7 +54,7 @@ TL_DEVICE f4 row4_load(const float* row, int d, int head_size) {
 template <bool VEC>
 TL_DEVICE void row4_store(float* row, int d, int head_size, f4 x) {
   if constexpr (VEC) {
-    *reinterpret_cast<f4*>(row + d) = x;
+    __builtin_nontemporal_store(x, reinterpret_cast<f4*>(row + d));
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -60,10 +62,37 @@ TL_DEVICE void row4_store(float* row, int d, int head_size, f4 x) {
   }
 }
 
-TL_DEVICE int byte_of(int x, int i) { return (int)(signed char)(x >> (8 * i)); }
+typedef int i4 __attribute__((ext_vector_type(4)));
 
-// The code of x under `scale`: 0 where the scale is 0 or NaN.
-TL_DEVICE int kv_code(float x, float scale) { return scale > 0.f ? q8_code(x, scale) : 0; }
+TL_DEVICE int byte_of(int x, int i) { return (int)(signed char)(x >> (8 * i)); }
+// The low bytes of four integers in one word.
+TL_DEVICE int pack4(int a, int b, int c, int d) {
+  const unsigned lo = __builtin_amdgcn_perm((unsigned)b, (unsigned)a, 0x0c0c0400u);
+  const unsigned hi = __builtin_amdgcn_perm((unsigned)d, (unsigned)c, 0x04000c0cu);
+  return (int)(lo | hi);
+}
+
+// Codes under one scale: round(x / scale), half away from zero, the quotient rounded to fp32 as if it were divided.
+// With both brought by the scale's power of two to where nothing over- or underflows (a quotient that loses bits
+// there is a code of 0), r = RN(1 / s), y = RN(x r), the remainder x - y s is exact and RN(y + r (x - y s)) is RN(x / s)
+// (Markstein; common.hpp q8_div_fast).  |x / s| <= 127 (1 + 2^-23), where truncating y + copysign(pred(0.5), y)
+// rounds half away.  A scale of 0 or NaN has codes of 0.
+struct KvCoder {
+  float s, r;
+  int e;
+  TL_DEVICE explicit KvCoder(float scale) {
+    const bool ok = scale > 0.f;
+    e = ok ? -__builtin_amdgcn_frexp_expf(scale) : 0;
+    s = ok ? __builtin_ldexpf(scale, e) : 0.f;
+    r = ok ? __fdiv_rn(1.f, s) : 0.f;
+  }
+  TL_DEVICE int operator()(float x) const {
+    x = __builtin_ldexpf(x, e);
+    const float y = __fmul_rn(x, r);
+    const float q = __builtin_fmaf(__builtin_fmaf(-y, s, x), r, y);
+    return (int)__fadd_rn(q, __builtin_copysignf(0.49999997f, q));
+  }
+};
 
 struct StoreArgs {
   Q8KVLayer l;
@@ -71,20 +100,25 @@ struct StoreArgs {
   const float* x[2];  // keys, values
   long long stride;
   int spanned;  // blocks that n_tokens rows may touch
+  int threads;  // of a head: block / 16 * lanes / 4
+  int heads;    // of a workgroup: several where one has less than a wave of threads
+  int groups;   // of heads
 };
 
-// One workgroup quantises what the call writes of one (keys or values, sequence, head, block of tokens):
-// thread (g, d4) the tokens 16g .. 16g + 15 of the block in dimensions 4*d4 .. + 3.
+// A workgroup quantises what the call writes of one (keys or values, sequence, block of tokens) and one or a few
+// heads: thread (head, g, d4) the tokens 16g .. 16g + 15 of the block in dimensions 4*d4 .. + 3, held in registers
+// between the maximum and the codes.  A group of one new token has code of its own: a decode step's store waits for
+// instructions as for anything else.
 template <bool VEC>
 __global__ void __launch_bounds__(512) k_q8kv_store(StoreArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
-  __shared__ unsigned red[8];
+  __shared__ unsigned red[16];
   const Q8KVLayer& l = a.l;
   unsigned u = blockIdx.x;
   const int jb = u % a.spanned;
   u /= a.spanned;
-  const int h = u % l.heads;
-  u /= l.heads;
+  const int hg = u % a.groups;
+  u /= a.groups;
   const int which = u & 1, b = u >> 1;
 
   long long row0;
@@ -92,88 +126,131 @@ __global__ void __launch_bounds__(512) k_q8kv_store(StoreArgs a) {
   q8kv_span(a.call, l.seq_len, b, row0, first, last);
   if (first >= last) return;
   const int j = (first >> l.block_log2) + jb;
-  const int start = j << l.block_log2;  // of the block; below first only in the first one
-  if (jb && start >= last) return;
+  const int start = j << l.block_log2, end = start + (1 << l.block_log2);
+  if (start >= last) return;
+  const int unit = threadIdx.x / a.threads, within = threadIdx.x - unit * a.threads;
   const int quads = l.lanes / 4;
-  const int g = threadIdx.x / quads, d = (threadIdx.x - g * quads) * 4;
+  const int g = within / quads, d = (within - g * quads) * 4;
   const int t0 = start + 16 * g;
-  const bool mine = (16 * g) >> l.block_log2 == 0;
-  const long long head = b * l.seq_codes + h * l.head_codes;
-  float* scale_p = (which ? l.vs : l.ks) + b * l.seq_scales + h * l.head_scales + j;
+  const int h = hg * a.heads + unit;
+  const bool mine = unit < a.heads && h < l.heads;
+  const bool full = first <= start && end <= last;
+  const long long head = b * l.seq_codes + (mine ? h : 0) * l.head_codes;
+  float* scale_p = (which ? l.vs : l.ks) + b * l.seq_scales + (mine ? h : 0) * l.head_scales + j;
+  const float* src = a.x[which] + (long long)h * l.head_size + ((long long)b * a.call.n_tokens + (t0 - row0)) * a.stride;
+  const bool earlier = start < first;
+  const float was = earlier ? *scale_p : 0.f;
 
-  // the rows: zeros where the call has none, and in dimensions from head_size on
-  f4 x[16];
-  const float* src = a.x[which] + (long long)h * l.head_size;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int t = t0 + i;
-    const bool in = mine && t >= first && t < last && d < l.head_size;
-    x[i] = in ? row4_load<VEC>(src + ((long long)b * a.call.n_tokens + (t - row0)) * a.stride, d, l.head_size)
-              : f4{0.f, 0.f, 0.f, 0.f};
-  }
   // |x| compared as integers: NaN above infinity above every number
+  auto largest = [](unsigned top, f4 x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    return top;
+  };
+  const int lo = max(first - t0, 0), hi = min(last - t0, 16);  // the group's new tokens
+  const bool one = hi - lo == 1;
+  f4 x[16];
+  x[0] = f4{0.f, 0.f, 0.f, 0.f};
   unsigned top = 0;
+  const bool live = mine && d < l.head_size;
+  if (one) {
+    if (live) x[0] = row4_load<VEC>(src + lo * a.stride, d, l.head_size);
+    top = largest(top, x[0]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 16; ++i) x[i] = live && i >= lo && i < hi ? row4_load<VEC>(src + i * a.stride, d, l.head_size) : f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
+    for (int i = 0; i < 16; ++i) top = largest(top, x[i]);
+  }
+  if (a.heads == 1) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-  __syncthreads();
-  for (unsigned w = 0; w < blockDim.x / 64; ++w) top = max(top, red[w]);
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();  // also: every thread has read the old scale
+    for (unsigned w = 0; w < blockDim.x / 64; ++w) top = max(top, red[w]);
+  } else {
+    if (threadIdx.x < 16) red[threadIdx.x] = 0;
+    __syncthreads();
+    if (mine) atomicMax(&red[unit], top);
+    __syncthreads();
+    top = mine ? red[unit] : 0;
+  }
 
   float scale = __fdiv_rn(__uint_as_float(top), 127.0f);
   if (scale < 1.17549435e-38f) scale = 0.f;
   if (top >= 0x7f800000u) scale = __builtin_nanf("");
-  const bool earlier = start < first;
-  float was = 0.f;
-  if (earlier) {
-    was = *scale_p;
-    if (!(scale > was) && scale == scale) scale = was;  // a NaN on either side stays
-  }
-  const bool again = earlier && !(scale == was);
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) *scale_p = scale;
-  if (!mine || t0 >= last || (t0 + 16 <= first && !again)) return;
+  if (earlier && !(scale > was) && scale == scale) scale = was;  // a NaN on either side stays
+  const bool again = earlier && !(scale == was);                 // earlier tokens change their codes
+  if (!mine) return;
+  if (within == 0) *scale_p = scale;
 
-  if (which == 0) {
-    int* dst = reinterpret_cast<int*>(l.k + head + (long long)t0 * l.lanes + d);
-    const int step = l.lanes / 4;
+  const KvCoder code(scale);
+  int* kd = reinterpret_cast<int*>(l.k + head + (long long)t0 * l.lanes + d);
+  i4* vd = reinterpret_cast<i4*>(l.v + head + (long long)t0 * l.lanes + (long long)d * 16);
+  const int step = l.lanes / 4;
+  if (full) {
+    if (which == 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = t0 + i;
-      if (t >= last || (t < first && !again)) continue;
-      int c[4];
-      if (t < first) {
-        const int old = dst[(long long)i * step];
+      for (int i = 0; i < 16; ++i) kd[i * step] = pack4(code(x[i][0]), code(x[i][1]), code(x[i][2]), code(x[i][3]));
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = kv_code(__fmul_rn((float)byte_of(old, e), was), scale);
-      } else {
+      for (int e = 0; e < 4; ++e) {
+        i4 w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = kv_code(x[i][e], scale);
+        for (int i = 0; i < 4; ++i) w[i] = pack4(code(x[4 * i][e]), code(x[4 * i + 1][e]), code(x[4 * i + 2][e]), code(x[4 * i + 3][e]));
+        vd[e] = w;
       }
-      dst[(long long)i * step] = (c[0] & 255) | (c[1] & 255) << 8 | (c[2] & 255) << 16 | c[3] << 24;
     }
-  } else {
-    typedef int i4 __attribute__((ext_vector_type(4)));
-    i4* dst = reinterpret_cast<i4*>(l.v + head + (long long)t0 * l.lanes + (long long)d * 16);
-    const bool whole = t0 >= first && t0 + 16 <= last;
+    return;
+  }
+  // codes of the tokens lo <= q .. q + 3 < hi
+  auto put = [&](int q, int lo, int hi, f4 y0, f4 y1, f4 y2, f4 y3) {
+    const f4 y[4] = {y0, y1, y2, y3};
+    if (which == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (q + i >= lo && q + i < hi) kd[(q + i) * step] = pack4(code(y[i][0]), code(y[i][1]), code(y[i][2]), code(y[i][3]));
+      return;
+    }
+    int8_t* at = reinterpret_cast<int8_t*>(vd) + q;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      i4 w = {0, 0, 0, 0};
-      if (!whole) w = dst[e];
+      const int w = pack4(code(y[0][e]), code(y[1][e]), code(y[2][e]), code(y[3][e]));
+      if (q >= lo && q + 4 <= hi) {
+        *reinterpret_cast<int*>(at + 16 * e) = w;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = t0 + i;
-        const int old = byte_of(w[i / 4], i % 4);
-        int c = old;
-        if (t >= first && t < last) c = kv_code(x[i][e], scale);
-        else if (t < first && again) c = kv_code(__fmul_rn((float)old, was), scale);
-        w[i / 4] = (w[i / 4] & ~(255 << (8 * (i % 4)))) | (c & 255) << (8 * (i % 4));
+        for (int i = 0; i < 4; ++i)
+          if (q + i >= lo && q + i < hi) at[16 * e + i] = (int8_t)byte_of(w, i);
       }
-      dst[e] = w;
     }
+  };
+  if (one) {  // a decode step's token
+    const int c[4] = {code(x[0][0]), code(x[0][1]), code(x[0][2]), code(x[0][3])};
+    if (which == 0) {
+      kd[lo * step] = pack4(c[0], c[1], c[2], c[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) reinterpret_cast<int8_t*>(vd)[16 * e + lo] = (int8_t)c[e];
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 16; q += 4)
+      if (q < hi && q + 4 > lo) put(q, lo, hi, x[q], x[q + 1], x[q + 2], x[q + 3]);
+  }
+  if (!again) return;
+#pragma unroll 1
+  for (int q = 0; q < min(lo, 16); q += 4) {
+    const int8_t* at = which ? reinterpret_cast<const int8_t*>(vd) + q : reinterpret_cast<const int8_t*>(kd + q * step);
+    int w[4];
+    f4 y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const int*>(at + i * (which ? 16 : l.lanes));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[i][e] = __fmul_rn((float)(which ? byte_of(w[e], i) : byte_of(w[i], e)), was);
+    put(q, 0, lo, y[0], y[1], y[2], y[3]);
   }
 }
 
@@ -218,7 +295,6 @@ __global__ void __launch_bounds__(256) k_q8kv_load(LoadArgs a, int both) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = t0 + i >= first && t0 + i < last ? src[(long long)i * (l.lanes / 4)] : 0;
   } else {
-    typedef int i4 __attribute__((ext_vector_type(4)));
     const i4* src = reinterpret_cast<const i4*>(l.v + head + d * 16);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -256,9 +332,12 @@ extern "C" thablasStatus_t thaDNN_q8_kv_store_batch(thablasHandle_t* handle, con
   const long long spanned = ((long long)n_tokens + c->block - 2) / c->block + 1;
   const long long most = (c->seq_len + (long long)c->block - 1) / c->block;
   a.spanned = (int)(spanned < most ? spanned : most);
-  const unsigned __int128 grid = (unsigned __int128)2 * n_batches * c->n_kv_heads * a.spanned;
+  a.threads = (c->block / 16) * (a.l.lanes / 4);
+  a.heads = a.threads < 64 ? 64 / a.threads : 1;
+  a.groups = (c->n_kv_heads + a.heads - 1) / a.heads;
+  const unsigned __int128 grid = (unsigned __int128)2 * n_batches * a.groups * a.spanned;
   if (grid > 0x7fffffff) return THABLAS_STATUS_NOT_SUPPORTED;
-  const int threads = ((c->block / 16) * (a.l.lanes / 4) + 63) / 64 * 64;
+  const int threads = (a.threads * a.heads + 63) / 64 * 64;
   tl::Q8KVDevice dev(handle->current_gpu_id);
   if (!dev.ok) return THABLAS_STATUS_INVALID_VALUE;
   auto kernel = tl::q8kv_vec4(c->head_size, kv_stride, k, v) ? tl::k_q8kv_store<true> : tl::k_q8kv_store<false>;
