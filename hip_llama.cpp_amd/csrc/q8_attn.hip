@@ -36,7 +36,8 @@ struct Q8AttnArgs {
   Q8KVCall call;
   const float* q;
   float* out;
-  float* part;  // nsplit > 1: [unit][split][row of the tile][head_size + 4] (sums, then M, sum of weights, E)
+  unsigned* arrived;  // nsplit > 1: [unit] workgroups that have left their part; 0 between calls
+  float* part;        // nsplit > 1: [unit][split][lrows][head_size rounded up to 4, + 4]
   long long q_stride, out_stride;
   int n_heads, mul;  // query heads, and how many of them share a K/V head
   int tiles;         // row tiles of a (sequence, K/V head)
@@ -90,38 +91,54 @@ struct AttnRows {
   float M, sum;  // running maximum, sum of weights
   f4 o[4 * KS];  // sums over the values: dimensions 16 d + 4 (lane >> 4) .. + 3
   int E;         // largest value exponent
+
+  TL_DEVICE void none() {  // before the first key
+    M = kNone;
+    sum = 0.f;
+    E = -126;
+#pragma unroll
+    for (int d = 0; d < 4 * KS; ++d) o[d] = f4{0.f, 0.f, 0.f, 0.f};
+  }
 };
 
-TL_DEVICE void attn_load_q(const Q8AttnArgs& a, const float* src, bool in, int d, float (&x)[16]) {
+// This lane's part of row r0 + (lane & 15) of the `rows` of (b, h), and the keys that the row sees.  A row behind the
+// last is the last one again; it sees what the tile sees and is never stored.  Every load is made, from inside the row, so that
+// none is waited for before the next is asked for.
+template <int KS>
+TL_DEVICE int attn_query(float (&x)[KS][16], const Q8AttnArgs& a, int b, int h, int r0, int rows, long long pos, int T) {
+  const int lane = threadIdx.x & 63, kg = lane >> 4, hs = a.l.head_size;
+  const int r = min(r0 + (lane & 15), rows - 1);
+  const int i = r / a.mul;
+  const long long p = pos + i;
+  const float* src = a.q + ((long long)b * a.call.n_tokens + i) * a.q_stride + (long long)(h * a.mul + r - i * a.mul) * hs;
   if (a.vec) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      f4 v = {0.f, 0.f, 0.f, 0.f};
-      if (in && d + e < a.l.head_size) v = *reinterpret_cast<const f4*>(src + d + e);
+    for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[e + c] = v[c];
-    }
+      for (int e = 0; e < 16; e += 4) {
+        const f4 v = *reinterpret_cast<const f4*>(src + min(64 * k + 16 * kg + e, hs - 4));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[k][e + c] = v[c];
+      }
   } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = in && d + e < a.l.head_size ? src[d + e] : 0.f;
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[k][e] = src[min(64 * k + 16 * kg + e, hs - 1)];
   }
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (64 * k + 16 * kg + e >= hs) x[k][e] = 0.f;
+  return r0 + (lane & 15) >= rows ? T : p >= 0 && p < a.l.seq_len ? (int)p + 1 : 0;
 }
 
-// Rows r0 .. r0 + 15 of the `rows` of (b, h).  A row behind the last sees what the tile sees and is never stored.
+// The query's digits.
 template <int KS>
-TL_DEVICE void attn_begin(AttnRows<KS>& s, const Q8AttnArgs& a, int b, int h, int r0, int rows, long long pos, int T) {
-  const int lane = threadIdx.x & 63, kg = lane >> 4;
-  const int r = r0 + (lane & 15);
-  const bool in = r < rows;
-  const int i = in ? r / a.mul : 0;
-  const long long p = pos + i;
-  s.seen = !in ? T : p >= 0 && p < a.l.seq_len ? (int)p + 1 : 0;
-  const float* src = a.q + ((long long)b * a.call.n_tokens + i) * a.q_stride +
-                     (long long)(h * a.mul + (in ? r - i * a.mul : 0)) * a.l.head_size;
-  float x[KS][16];
+TL_DEVICE void attn_begin(AttnRows<KS>& s, const float (&x)[KS][16], int seen) {
+  s.seen = seen;
   unsigned top = 0;
-#pragma unroll
-  for (int k = 0; k < KS; ++k) attn_load_q(a, src, in, 64 * k + 16 * kg, x[k]);
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -142,11 +159,6 @@ TL_DEVICE void attn_begin(AttnRows<KS>& s, const Q8AttnArgs& a, int b, int h, in
       s.q[1][k][e] = p1;
       s.q[2][k][e] = p2;
     }
-  s.M = kNone;
-  s.sum = 0.f;
-#pragma unroll
-  for (int d = 0; d < 4 * KS; ++d) s.o[d] = f4{0.f, 0.f, 0.f, 0.f};
-  s.E = -126;
 }
 
 // Scales of this lane's sixteen keys in each of NT tiles of 64 from t0 on; those of keys that nobody sees are 0.
@@ -327,8 +339,8 @@ struct AttnUnit {  // what a workgroup works on
 TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, AttnUnit& w) {
   w.h = pair % a.l.heads;
   w.b = pair / a.l.heads;
-  const int count = a.call.n_d ? min(max(a.call.n_d[w.b], 0), a.call.n_tokens) : a.call.n_tokens;
-  w.pos = a.call.pos_d[w.b];
+  int count;
+  q8kv_start(a.call, w.b, w.pos, count);
   w.rows = count * a.mul;
   w.r0 = tile * R;
   if (w.r0 >= w.rows) return false;
@@ -375,12 +387,40 @@ TL_DEVICE void lds_wait() {
   __syncthreads();
 }
 
-// Few rows: one workgroup takes 16 query rows of one (sequence, K/V head) and, of their keys, every nsplit-th run of
-// a 64-key tile for each of its waves; the waves' results are joined in LDS, the workgroups' by k_q8_attn_join.
+// A tile of 64 keys as one wave holds it.
 template <int KS>
-__global__ void __launch_bounds__(KS < 4 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a) {
+struct AttnTile {
+  i4 k[4][KS], v[4 * KS];
+  AttnScales<1> c;
+  TL_DEVICE void load_keys(const Q8AttnArgs& a, const int8_t* k0, const float* ks, const float* vs, int t0, int T) {
+    const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+    const int8_t* kp = k0 + (long long)(t0 + 16 * (row >> 2) + (row & 3)) * a.l.lanes;
+    c.load(a, ks, vs, t0, T);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int d = 0; d < KS; ++d) {
+        const int at = 64 * d + 16 * g;
+        k[j][d] = *reinterpret_cast<const i4*>(kp + 4 * j * a.l.lanes + (at < a.l.lanes ? at : 0));  // the query's digits are 0 from lanes on
+      }
+  }
+  TL_DEVICE void load_values(const Q8AttnArgs& a, const int8_t* v0, int t0) {
+    const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+    const int8_t* vp = v0 + (long long)((t0 >> 4) + g) * (16 * a.l.lanes) + 16 * row;
+#pragma unroll
+    for (int d = 0; d < 4 * KS; ++d) v[d] = *reinterpret_cast<const i4*>(vp + (16 * d < a.l.lanes ? 256 * d : 0));
+  }
+};
+
+// Few rows: one workgroup takes 16 query rows of one (sequence, K/V head) and, of their keys, every nsplit-th run of
+// a 64-key tile for each of its waves.  A wave asks for its next keys as soon as the scores are done with these, and for
+// its next values when the sums are.  The waves' results are joined in LDS; where several workgroups share a row tile, each leaves its result in the workspace and the last
+// one to arrive joins them, in the order of the splits whoever it is.
+template <int KS>
+__global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
   extern __shared__ __attribute__((aligned(16))) float lds[];
+  __shared__ int last;
   const Q8KVLayer& l = a.l;
   unsigned u = blockIdx.x;
   const int split = u % a.nsplit;
@@ -389,39 +429,41 @@ __global__ void __launch_bounds__(KS < 4 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
   if (!attn_unit(a, unit % pairs, a.tiles - 1 - unit / pairs, 16, w)) return;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-  AttnRows<KS> s;
-  attn_begin<KS>(s, a, w.b, w.h, w.r0, w.rows, w.pos, w.T);
-  const int least = attn_least(s.seen);
   const int8_t* k = l.k + w.b * l.seq_codes + w.h * l.head_codes;
   const int8_t* v = l.v + w.b * l.seq_codes + w.h * l.head_codes;
   const float* ks = l.ks + w.b * l.seq_scales + w.h * l.head_scales;
   const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
   const int row = lane & 15, g = lane >> 4;
-  for (int t0 = 64 * (split * waves + wave); t0 < w.T; t0 += 64 * waves * a.nsplit) {
-    const int8_t* kp = k + (long long)(t0 + 16 * (row >> 2) + (row & 3)) * l.lanes;
-    const int8_t* vp = v + (long long)((t0 >> 4) + g) * (16 * l.lanes) + 16 * row;
-    i4 kc[4][KS], vc[4 * KS];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int c = 0; c < KS; ++c) {
-        const int d = 64 * c + 16 * g;
-        kc[j][c] = *reinterpret_cast<const i4*>(kp + 4 * j * l.lanes + (d < l.lanes ? d : 0));  // the query's digits are 0 from lanes on
-      }
-    AttnScales<1> sc;
-    sc.load(a, ks, vs, t0, w.T);
-#pragma unroll
-    for (int d = 0; d < 4 * KS; ++d)
-      vc[d] = *reinterpret_cast<const i4*>(vp + (16 * d < l.lanes ? 256 * d : 0));
-    attn_step<KS, 1>(s, a, sc, t0, t0 + 64 > least, [&](int, int j, int c) { return kc[j][c]; }, [&](int, int d) { return vc[d]; }, [] {});
+  const int step = 64 * waves * a.nsplit;
+  int t0 = 64 * (split * waves + wave);
+  AttnRows<KS> s;
+  s.none();
+  if (t0 < w.T) {
+    AttnTile<KS> tile;
+    {
+      float x[KS][16];
+      const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0, w.rows, w.pos, w.T);
+      tile.load_keys(a, k, ks, vs, t0, w.T);
+      tile.load_values(a, v, t0);
+      attn_begin<KS>(s, x, seen);
+    }
+    const int least = attn_least(s.seen);
+    auto key = [&](int, int j, int d) { return tile.k[j][d]; };
+    auto val = [&](int, int d) { return tile.v[d]; };
+    for (; t0 + step < w.T; t0 += step) {
+      AttnScales<1> c = tile.c;
+      attn_step<KS, 1>(s, a, c, t0, t0 + 64 > least, key, val, [&] { tile.load_keys(a, k, ks, vs, t0 + step, w.T); });
+      tile.load_values(a, v, t0 + step);
+    }
+    attn_step<KS, 1>(s, a, tile.c, t0, t0 + 64 > least, key, val, [] {});
   }
 
   // join the waves' rows
-  const int hs = l.head_size, step = 64 * KS + 4;
-  float* stat = lds + waves * a.lrows * step;
+  const int hs = l.head_size, wide = 64 * KS + 4;
+  float* stat = lds + waves * a.lrows * wide;
   s.sum = rows_sum(s.sum);
   if (row < w.nr) {
-    float* dst = lds + (wave * a.lrows + row) * step + 4 * g;
+    float* dst = lds + (wave * a.lrows + row) * wide + 4 * g;
 #pragma unroll
     for (int d = 0; d < 4 * KS; ++d) *reinterpret_cast<f4*>(dst + 16 * d) = s.o[d];
     if (lane < 16) {
@@ -432,8 +474,11 @@ __global__ void __launch_bounds__(KS < 4 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
   }
   __syncthreads();
   const int quads = (hs + 3) / 4;
+  const __amdgpu_buffer_rsrc_t parts = rsrc_of(a.part);
+  const unsigned part = 16u * (quads + 1);                // bytes of a row's part: sums, then M, sum of weights, E
+  const unsigned mine = unit * a.nsplit * a.lrows * part;  // of the unit's first
   for (int it = threadIdx.x; it < w.nr * quads; it += blockDim.x) {
-    const int r = it / quads, d = (it - r * quads) * 4;
+    const int r = it / quads, d = it - r * quads;
     float M = kNone, E = -126.f;
     for (int n = 0; n < waves; ++n) {
       M = fmaxf(M, stat[3 * (n * a.lrows + r)]);
@@ -445,24 +490,67 @@ __global__ void __launch_bounds__(KS < 4 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
       const float* st = stat + 3 * (n * a.lrows + r);
       float wo, ws;
       row_join(M, E, {st[0], st[1], st[2]}, wo, ws);
-      const f4 x = *reinterpret_cast<const f4*>(lds + (n * a.lrows + r) * step + d);
+      const f4 x = *reinterpret_cast<const f4*>(lds + (n * a.lrows + r) * wide + 4 * d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], wo, o[e]);
       sum += ws;
     }
-    if (a.nsplit > 1) {
-      float* dst = a.part + (((long long)unit * a.nsplit + split) * 16 + r) * (hs + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (d + e < hs) dst[d + e] = o[e];
-      if (d == 0) {
-        dst[hs] = M;
-        dst[hs + 1] = sum;
-        dst[hs + 2] = E;
-      }
-    } else {
-      attn_store(a, w, r, d, o, M, sum, E);
+    if (a.nsplit == 1) {
+      attn_store(a, w, r, 4 * d, o, M, sum, E);
+      continue;
     }
+    const unsigned at = mine + (split * a.lrows + r) * part;
+    st4_sc1(parts, at + 16 * d, o);
+    if (d == 0) st4_sc1(parts, at + 16 * quads, f4{M, sum, E, 0.f});
+  }
+  if (a.nsplit == 1) return;
+
+  // Parts are written through and read past the caches of the XCDs (sc1); each wave's have arrived before the count.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned before = __hip_atomic_fetch_add(&a.arrived[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = before == (unsigned)a.nsplit - 1;
+    if (last) __hip_atomic_store(&a.arrived[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
+  for (int it = threadIdx.x; it < w.nr * quads; it += blockDim.x) {
+    const int r = it / quads, d = it - r * quads;
+    const unsigned at = mine + r * part, stride = a.lrows * part;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    float M = kNone, E = -126.f, sum = 0.f;
+    for (int n0 = 0; n0 < a.nsplit; n0 += 8) {  // eight parts under way at once, each joined to what is before it
+      f4 x[8], st[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const unsigned p = at + min(n0 + n, a.nsplit - 1) * stride;
+        st[n] = ld4_sc1(parts, p + 16 * quads);
+        x[n] = ld4_sc1(parts, p + 16 * d);
+      }
+      float m = M, e8 = E;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        m = fmaxf(m, st[n].x);
+        e8 = fmaxf(e8, st[n].z);
+      }
+      float wo, ws;
+      row_join(m, e8, {M, sum, E}, wo, ws);
+      sum = ws;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= wo;
+      M = m;
+      E = e8;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        if (n0 + n >= a.nsplit) continue;
+        row_join(M, E, {st[n].x, st[n].y, st[n].z}, wo, ws);
+        sum += ws;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[n][e], wo, o[e]);
+      }
+    }
+    attn_store(a, w, r, 4 * d, o, M, sum, E);
   }
 }
 
@@ -509,7 +597,12 @@ __global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs
 
   if (w.T > 0) keys_in(0);
   AttnRows<KS> s;
-  attn_begin<KS>(s, a, w.b, w.h, w.r0 + 16 * wave, w.rows, w.pos, w.T);
+  s.none();
+  {
+    float x[KS][16];
+    const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0 + 16 * wave, w.rows, w.pos, w.T);
+    attn_begin<KS>(s, x, seen);
+  }
   const int least = attn_least(s.seen);
   const int most = -attn_least(-s.seen);
   for (int t0 = 0; t0 < w.T; t0 += 64 * NT) {
@@ -535,39 +628,10 @@ __global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs
       if (16 * d + 4 * g < l.head_size) attn_store(a, w, 16 * wave + row, 16 * d + 4 * g, s.o[d], s.M, s.sum, (float)s.E);
 }
 
-// Joins the splits of one (row tile, row): one wave each, lanes along the dimensions.
-__global__ void __launch_bounds__(64) k_q8_attn_join(Q8AttnArgs a, int R) {
-  keep_implicit_args();  // common.hpp
-  const int lane = threadIdx.x, hs = a.l.head_size;
-  const int r = blockIdx.x % R;
-  const unsigned unit = blockIdx.x / R, pairs = a.call.n_batches * a.l.heads;
-  const int tile = a.tiles - 1 - unit / pairs, h = unit % pairs % a.l.heads, b = unit % pairs / a.l.heads;
-  const int count = a.call.n_d ? min(max(a.call.n_d[b], 0), a.call.n_tokens) : a.call.n_tokens;
-  const int row = tile * R + r;
-  if (row >= count * a.mul) return;
-  const float* src = a.part + ((long long)unit * a.nsplit * R + r) * (hs + 4);
-  const long long step = (long long)R * (hs + 4);
-  float M = kNone, E = -126.f;
-  for (int s = 0; s < a.nsplit; ++s) {
-    M = fmaxf(M, src[s * step + hs]);
-    E = fmaxf(E, src[s * step + hs + 2]);
-  }
-  const int i = row / a.mul;
-  float* dst = a.out + ((long long)b * a.call.n_tokens + i) * a.out_stride + (long long)(h * a.mul + row - i * a.mul) * hs;
-  for (int d = lane; d < hs; d += 64) {
-    float o = 0.f, sum = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float* st = src + s * step + hs;
-      float wo, ws;
-      row_join(M, E, {st[0], st[1], st[2]}, wo, ws);
-      o = fmaf(src[s * step + d], wo, o);
-      sum += ws;
-    }
-    dst[d] = M == kNone && sum == 0.f ? 0.f : __builtin_ldexpf(o / (sum * kDigits), (int)E);
-  }
-}
+constexpr int kAttnBlocks = 512;        // workgroups that keep the card's 256 CUs busy
+constexpr int kAttnUnits = kAttnBlocks / 2;  // row tiles that are divided among workgroups, at most
 
-constexpr int kAttnBlocks = 512;  // workgroups that keep the card's 256 CUs busy
+inline size_t attn_part(int head_size) { return 16 * ((head_size + 3) / 4 + 1); }  // bytes of a row's part
 
 // How a call's rows and keys are divided.
 struct AttnPlan {
@@ -581,7 +645,7 @@ static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n
   p.many = pairs * ((rows + 63) / 64) >= kAttnBlocks / 2 && rows >= 64;
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
-  p.waves = p.many || c->head_size > 192 ? 4 : 8;
+  p.waves = p.many || c->head_size > 128 ? 4 : 8;
   const long long most = (c->seq_len + 64LL * p.waves - 1) / (64 * p.waves);  // every wave has a tile to do
   p.nsplit = p.many ? 1 : (int)max(1LL, min(most, min(64LL, kAttnBlocks / p.units)));
   return p;
@@ -596,7 +660,7 @@ static hipError_t attn_launch(const Q8AttnArgs& a, const AttnPlan& p, hipStream_
   }
   const size_t lds = (size_t)p.waves * a.lrows * (64 * KS + 4 + 3) * sizeof(float);
   if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)k_q8_attn_few<KS>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    const hipError_t e = hipFuncSetAttribute((const void*)k_q8_attn_few<KS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL((k_q8_attn_few<KS>), grid, block, lds, s, a);
@@ -613,10 +677,8 @@ extern "C" size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batche
   if (!c || n_batches <= 0 || n_tokens <= 0 || !tl::q8kv_sizes_ok(c->n_batches, c->n_layers, c->n_kv_heads, c->head_size, c->seq_len) ||
       !tl::q8kv_supported(c->head_size, c->block) || !attn_sizes_ok(c, n_heads))
     return 0;
-  // a call of fewer rows may split its keys among more workgroups, but never has more than this many parts
-  const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads), units = (long long)n_batches * c->n_kv_heads * ((rows + 15) / 16);
-  const long long parts = units < tl::kAttnBlocks ? units * 64 : tl::kAttnBlocks;
-  return (size_t)(parts < tl::kAttnBlocks ? parts : tl::kAttnBlocks) * 16 * (c->head_size + 4) * sizeof(float);
+  // a call of fewer rows may divide its keys among more workgroups, but never has more than this many parts
+  return tl::kAttnUnits * sizeof(unsigned) + (size_t)tl::kAttnBlocks * 16 * tl::attn_part(c->head_size);
 }
 
 extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, const Q8KVCache* c, int layer,
@@ -634,19 +696,21 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   const int mul = n_heads / c->n_kv_heads;
   const tl::AttnPlan p = tl::attn_plan(c, n_batches, n_tokens, n_heads);
   if ((long long)n_tokens * mul > 0x7fffffffLL - 64 || p.units * p.nsplit > 0x7fffffffLL / 16) return THABLAS_STATUS_NOT_SUPPORTED;
-  const size_t need = p.nsplit > 1 ? (size_t)p.units * p.nsplit * 16 * (c->head_size + 4) * sizeof(float) : 0;
+  const int lrows = (int)min((long long)n_tokens * mul, 16LL);
+  const size_t need = p.nsplit > 1 ? tl::kAttnUnits * sizeof(unsigned) + (size_t)p.units * p.nsplit * lrows * tl::attn_part(c->head_size) : 0;
   if (need && (!work || ((uintptr_t)work & 15) || work_bytes < need)) return THABLAS_STATUS_INVALID_VALUE;
   a.call = {pos_d, n_d, n_batches, n_tokens};
   a.q = q;
   a.out = out;
-  a.part = static_cast<float*>(work);
+  a.arrived = static_cast<unsigned*>(work);
+  a.part = reinterpret_cast<float*>(a.arrived + tl::kAttnUnits);
   a.q_stride = q_stride;
   a.out_stride = out_stride;
   a.n_heads = n_heads;
   a.mul = mul;
   a.tiles = (int)p.tiles;
   a.nsplit = p.nsplit;
-  a.lrows = (int)min((long long)n_tokens * mul, 16LL);
+  a.lrows = lrows;
   a.vec = tl::q8kv_vec4(c->head_size, q_stride, q, out) && out_stride % 4 == 0;
   a.c0 = (float)(1.4426950408889634 / __builtin_sqrt((double)c->head_size) / tl::kDigits);
   tl::Q8KVDevice dev(handle->current_gpu_id);
@@ -659,7 +723,5 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   else if (ks == 3) e = tl::attn_launch<3>(a, p, s);
   else e = tl::attn_launch<4>(a, p, s);
   if (e != hipSuccess) return THABLAS_STATUS_EXECUTION_FAILED;
-  if (p.nsplit > 1)
-    hipLaunchKernelGGL(tl::k_q8_attn_join, dim3((unsigned)(p.units * 16)), dim3(64), 0, s, a, 16);
-  return tl::q8kv_status(hipGetLastError());
+  return THABLAS_STATUS_SUCCESS;
 }

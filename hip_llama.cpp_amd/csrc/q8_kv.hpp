@@ -28,10 +28,18 @@ struct Q8KVCall {
   int n_batches, n_tokens;
 };
 
-// Positions [first, last) of sequence b's rows, clipped to the cache; `row0` is the position of its row 0.
+// The position of sequence b's row 0 and the number of its rows, asked for at once by scalar loads.
+TL_DEVICE void q8kv_start(const Q8KVCall& call, int b, long long& row0, int& n) {
+  typedef const __attribute__((address_space(4))) int* scalar;
+  const int* count = call.n_d ? call.n_d : call.pos_d;
+  const int p = ((scalar)(uintptr_t)call.pos_d)[b], c = ((scalar)(uintptr_t)count)[b];
+  row0 = p;
+  n = call.n_d ? min(max(c, 0), call.n_tokens) : call.n_tokens;
+}
+// Positions [first, last) of sequence b's rows, clipped to the cache.
 TL_DEVICE void q8kv_span(const Q8KVCall& call, int seq_len, int b, long long& row0, int& first, int& last) {
-  const int n = call.n_d ? min(max(call.n_d[b], 0), call.n_tokens) : call.n_tokens;
-  row0 = call.pos_d[b];
+  int n;
+  q8kv_start(call, b, row0, n);
   first = (int)max(row0, 0LL);
   last = (int)max(0LL, min(row0 + n, (long long)seq_len));
 }

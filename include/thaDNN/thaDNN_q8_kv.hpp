@@ -61,16 +61,17 @@ thablasStatus_t thaDNN_q8_kv_load_batch(thablasHandle_t* handle, const Q8KVCache
                                         int n_tokens, const int* pos_d, const int* n_d, float* k, float* v,
                                         int kv_stride);
 
-// Bytes of workspace that thaDNN_q8_attention_batch needs for up to n_batches sequences of up to n_tokens rows
-// (0: none; also for arguments that the call refuses).
+// Bytes of workspace that thaDNN_q8_attention_batch may use for the cache's sequences, whatever their number and rows
+// (0 for arguments that the call refuses).
 size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads);
 
 // Causal attention of n_heads query heads over the cache, query head h with K/V head h / (n_heads / n_kv_heads):
 //   out_i[h] = sum_{t <= p} softmax_t(q_i[h] . k_t / sqrtf(head_size)) v_t,   p = pos_d[b] + i
 // in fp32's accuracy.  A decode step is n_tokens = 1 after its token's store, a prompt's chunk n_tokens > 1.
 // A row at a position outside 0 .. seq_len - 1 sees no key: zeros.  Rows from n_d[b] on are left as they were.
-// q and out are [n_batches][n_tokens][n_heads * head_size] and do not overlap.  work (16-byte aligned) belongs to
-// the call until its kernels have run: calls that may run at once have one each.  It need not be set.
+// q and out are [n_batches][n_tokens][n_heads * head_size] and do not overlap.  work (16-byte aligned) is zeroed once,
+// before its first call (thallama_memset), and then left to these calls, of any shape: each leaves it ready for the next.  It
+// belongs to a call until its kernel has run: calls that may run at once, captured ones among them, have one each.
 thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, const Q8KVCache* c, int layer, int n_batches,
                                           int n_tokens, const int* pos_d, const int* n_d, int n_heads,
                                           const float* q, float* out, int q_stride, int out_stride, void* work,

@@ -54,7 +54,7 @@ BAD = [(dict(handle=False), NULL_HANDLE), (dict(cache=False), INVALID), (dict(gp
        (dict(hs=0), INVALID), (dict(S=0), INVALID), (dict(block=0), INVALID), (dict(B=0), INVALID), (dict(L=-2), INVALID),
        (dict(H=-4), INVALID), (dict(B=1 << 30, L=1 << 30, H=1 << 20, nb=1), INVALID), (dict(nb=0), OK), (dict(n=0), OK),
        (dict(nb=0, pos=None, x=None, y=None), OK), (dict(x=AT + 2), INVALID), (dict(y=AT + 1), INVALID)]
-BIG = dict(B=1 << 24, L=1, H=64, hs=16, S=16, block=16, nb=1 << 24, layer=0, n=16)  # more workgroups than a launch holds
+BIG = dict(B=1 << 24, L=1, H=64, hs=256, S=16, block=16, nb=1 << 24, layer=0, n=16)  # more workgroups than a launch holds
 
 
 def call(tl, op, **change):
@@ -76,10 +76,10 @@ def test_refusals(tl, op, change, status):
 @pytest.mark.parametrize("op,change,status", [
     ("store", dict(x=None), INVALID), ("store", dict(y=None), INVALID), ("store", dict(stride=255), INVALID),
     ("store", dict(stride=-1), INVALID), ("load", dict(stride=255), INVALID), ("load", dict(x=None, y=None), OK),
-    ("store", dict(BIG, stride=1024), UNSUPPORTED), ("load", dict(BIG, B=1 << 30, nb=1 << 30, H=1, stride=16), UNSUPPORTED),
+    ("store", dict(BIG, stride=16384), UNSUPPORTED), ("load", dict(BIG, B=1 << 30, nb=1 << 30, H=1, hs=16, stride=16), UNSUPPORTED),
     ("attention", dict(x=None), INVALID), ("attention", dict(y=None), INVALID), ("attention", dict(qstride=511), INVALID),
     ("attention", dict(ostride=511), INVALID), ("attention", dict(heads=0), INVALID), ("attention", dict(heads=6), INVALID),
-    ("attention", dict(heads=-4), INVALID), ("attention", dict(BIG, heads=64, qstride=1024, ostride=1024, n=1 << 20), UNSUPPORTED)])
+    ("attention", dict(heads=-4), INVALID), ("attention", dict(BIG, heads=64, qstride=16384, ostride=16384, n=1 << 20), UNSUPPORTED)])
 def test_refusals_of_one(tl, op, change, status):
     assert call(tl, op, **change) == status
 

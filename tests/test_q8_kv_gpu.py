@@ -80,7 +80,7 @@ class Device:
         dq = self.gpu.DevBuf.from_array(np.concatenate([np.full(shift, np.nan, np.float32), full.ravel()]))
         out = self.gpu.DevBuf.from_array(np.full(shift + full.size, -77.0, np.float32))
         size = self.lib.thaDNN_q8_attention_workspace(C.byref(self.c), B, nt, heads)
-        work = self.gpu.DevBuf.from_array(np.full(max(size, 1), 255, np.uint8))
+        work = self.gpu.DevBuf.from_array(np.zeros(max(size, 1), np.uint8))
         p, m = self.ints(pos), self.ints(n)
         rc = self.lib.thaDNN_q8_attention_batch(C.byref(handle or self.handle), C.byref(self.c), layer, B, nt, p.ptr, m and m.ptr,
                                                 heads, dq.ptr + 4 * shift, out.ptr + 4 * shift, row + pad, row + pad, work.ptr, size)
@@ -441,7 +441,7 @@ def test_captured_decode_step(gpu):
     size = dev.lib.thaDNN_q8_attention_workspace(C.byref(dev.c), B, 1, H * mul)
     pos = dev.ints([900, 40])
     k, v, q = gpu.DevBuf(B * row * 4), gpu.DevBuf(B * row * 4), gpu.DevBuf(B * row * mul * 4)
-    out, work = gpu.DevBuf(B * row * mul * 4), gpu.DevBuf(max(size, 1))
+    out, work = gpu.DevBuf(B * row * mul * 4), gpu.DevBuf.from_array(np.zeros(size, np.uint8))
 
     def step():
         h, c = C.byref(handle), C.byref(dev.c)
@@ -477,7 +477,7 @@ def test_two_streams_at_once(gpu):
     alone = [dev.attend(0, [999, 600], None, q) for q in qs]
     size = dev.lib.thaDNN_q8_attention_workspace(C.byref(dev.c), B, 1, H)
     pos = dev.ints([999, 600])
-    bufs = [[gpu.DevBuf.from_array(q), gpu.DevBuf(q.nbytes), gpu.DevBuf(max(size, 1))] for q in qs]
+    bufs = [[gpu.DevBuf.from_array(q), gpu.DevBuf(q.nbytes), gpu.DevBuf.from_array(np.zeros(size, np.uint8))] for q in qs]
     gpu.sync()
     for _ in range(20):
         for h, (q, out, work) in zip(handles, bufs):
