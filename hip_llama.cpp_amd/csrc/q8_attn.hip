@@ -30,6 +30,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
 constexpr float kNone = -1e30f;       // a maximum over nothing
+constexpr int kWaves = 8;             // of a workgroup, at most
 
 struct Q8AttnArgs {
   Q8KVLayer l;
@@ -126,19 +127,20 @@ TL_DEVICE int attn_query(float (&x)[KS][16], const Q8AttnArgs& a, int b, int h, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[k][e] = src[min(64 * k + 16 * kg + e, hs - 1)];
   }
-#pragma unroll
-  for (int k = 0; k < KS; ++k)
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (64 * k + 16 * kg + e >= hs) x[k][e] = 0.f;
   return r0 + (lane & 15) >= rows ? T : p >= 0 && p < a.l.seq_len ? (int)p + 1 : 0;
 }
 
 // The query's digits.
 template <int KS>
-TL_DEVICE void attn_begin(AttnRows<KS>& s, const float (&x)[KS][16], int seen) {
+TL_DEVICE void attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen) {
   s.seen = seen;
+  const int left = hs - 16 * ((threadIdx.x & 63) >> 4);
   unsigned top = 0;
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (64 * k + e >= left) x[k][e] = 0.f;
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -350,13 +352,32 @@ TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, At
   return true;
 }
 
-// What a wave, a workgroup or a split knows of a row: sum_t 2^(x_t) v_t = 2^M o and sum_t 2^(x_t) = 2^(M - E) sum.
-struct RowPart {
-  float M, sum, E;
-};
-TL_DEVICE void row_join(float M, float E, const RowPart& r, float& wo, float& ws) {
-  wo = __builtin_amdgcn_exp2f(r.M - M);
-  ws = r.sum == 0.f ? 0.f : __builtin_amdgcn_exp2f((r.M - M) + (E - r.E)) * r.sum;
+// A wave, a workgroup or a split knows of a row sum_t 2^(x_t) v_t = 2^M o and sum_t 2^(x_t) = 2^(M - E) sum.  Joins the
+// first n of N such parts, st = (M, sum, E), to one.
+template <int N>
+TL_DEVICE void parts_join(const f4 (&x)[N], const f4 (&st)[N], int n, f4& o, float& M, float& sum, float& E) {
+  float m = M, top = E;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i >= n) continue;
+    m = fmaxf(m, st[i].x);
+    top = fmaxf(top, st[i].z);
+  }
+  auto weight = [&](float M1, float sum1, float E1) { return sum1 == 0.f ? 0.f : __builtin_amdgcn_exp2f((M1 - m) + (top - E1)) * sum1; };
+  sum = weight(M, sum, E);
+  const float w = __builtin_amdgcn_exp2f(M - m);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= w;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i >= n) continue;
+    sum += weight(st[i].x, st[i].y, st[i].z);
+    const float wi = __builtin_amdgcn_exp2f(st[i].x - m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], wi, o[e]);
+  }
+  M = m;
+  E = top;
 }
 
 // Dimensions d .. d + 3 of row r of the unit, from its sums.  A row without keys is zeros.
@@ -401,14 +422,14 @@ struct AttnTile {
 #pragma unroll
       for (int d = 0; d < KS; ++d) {
         const int at = 64 * d + 16 * g;
-        k[j][d] = *reinterpret_cast<const i4*>(kp + 4 * j * a.l.lanes + (at < a.l.lanes ? at : 0));  // the query's digits are 0 from lanes on
+        k[j][d] = __builtin_nontemporal_load(reinterpret_cast<const i4*>(kp + 4 * j * a.l.lanes + (at < a.l.lanes ? at : 0)));  // the query's digits are 0 from lanes on
       }
   }
   TL_DEVICE void load_values(const Q8AttnArgs& a, const int8_t* v0, int t0) {
     const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
     const int8_t* vp = v0 + (long long)((t0 >> 4) + g) * (16 * a.l.lanes) + 16 * row;
 #pragma unroll
-    for (int d = 0; d < 4 * KS; ++d) v[d] = *reinterpret_cast<const i4*>(vp + (16 * d < a.l.lanes ? 256 * d : 0));
+    for (int d = 0; d < 4 * KS; ++d) v[d] = __builtin_nontemporal_load(reinterpret_cast<const i4*>(vp + (16 * d < a.l.lanes ? 256 * d : 0)));
   }
 };
 
@@ -445,7 +466,7 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
       const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0, w.rows, w.pos, w.T);
       tile.load_keys(a, k, ks, vs, t0, w.T);
       tile.load_values(a, v, t0);
-      attn_begin<KS>(s, x, seen);
+      attn_begin<KS>(s, x, a.l.head_size, seen);
     }
     const int least = attn_least(s.seen);
     auto key = [&](int, int j, int d) { return tile.k[j][d]; };
@@ -460,17 +481,13 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
 
   // join the waves' rows
   const int hs = l.head_size, wide = 64 * KS + 4;
-  float* stat = lds + waves * a.lrows * wide;
+  f4* stat = reinterpret_cast<f4*>(lds + waves * a.lrows * wide);
   s.sum = rows_sum(s.sum);
   if (row < w.nr) {
     float* dst = lds + (wave * a.lrows + row) * wide + 4 * g;
 #pragma unroll
     for (int d = 0; d < 4 * KS; ++d) *reinterpret_cast<f4*>(dst + 16 * d) = s.o[d];
-    if (lane < 16) {
-      stat[3 * (wave * a.lrows + row)] = s.M;
-      stat[3 * (wave * a.lrows + row) + 1] = s.sum;
-      stat[3 * (wave * a.lrows + row) + 2] = (float)s.E;
-    }
+    if (lane < 16) stat[wave * a.lrows + row] = f4{s.M, s.sum, (float)s.E, 0.f};
   }
   __syncthreads();
   const int quads = (hs + 3) / 4;
@@ -479,22 +496,16 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
   const unsigned mine = unit * a.nsplit * a.lrows * part;  // of the unit's first
   for (int it = threadIdx.x; it < w.nr * quads; it += blockDim.x) {
     const int r = it / quads, d = it - r * quads;
-    float M = kNone, E = -126.f;
-    for (int n = 0; n < waves; ++n) {
-      M = fmaxf(M, stat[3 * (n * a.lrows + r)]);
-      E = fmaxf(E, stat[3 * (n * a.lrows + r) + 2]);
+    f4 x[kWaves], st[kWaves];
+#pragma unroll
+    for (int n = 0; n < kWaves; ++n) {
+      const int at = min(n, waves - 1) * a.lrows + r;
+      st[n] = stat[at];
+      x[n] = *reinterpret_cast<const f4*>(lds + at * wide + 4 * d);
     }
     f4 o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    for (int n = 0; n < waves; ++n) {
-      const float* st = stat + 3 * (n * a.lrows + r);
-      float wo, ws;
-      row_join(M, E, {st[0], st[1], st[2]}, wo, ws);
-      const f4 x = *reinterpret_cast<const f4*>(lds + (n * a.lrows + r) * wide + 4 * d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], wo, o[e]);
-      sum += ws;
-    }
+    float M = kNone, E = -126.f, sum = 0.f;
+    parts_join(x, st, waves, o, M, sum, E);
     if (a.nsplit == 1) {
       attn_store(a, w, r, 4 * d, o, M, sum, E);
       continue;
@@ -528,27 +539,7 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
         st[n] = ld4_sc1(parts, p + 16 * quads);
         x[n] = ld4_sc1(parts, p + 16 * d);
       }
-      float m = M, e8 = E;
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        m = fmaxf(m, st[n].x);
-        e8 = fmaxf(e8, st[n].z);
-      }
-      float wo, ws;
-      row_join(m, e8, {M, sum, E}, wo, ws);
-      sum = ws;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= wo;
-      M = m;
-      E = e8;
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        if (n0 + n >= a.nsplit) continue;
-        row_join(M, E, {st[n].x, st[n].y, st[n].z}, wo, ws);
-        sum += ws;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[n][e], wo, o[e]);
-      }
+      parts_join(x, st, a.nsplit - n0, o, M, sum, E);
     }
     attn_store(a, w, r, 4 * d, o, M, sum, E);
   }
@@ -601,7 +592,7 @@ __global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs
   {
     float x[KS][16];
     const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0 + 16 * wave, w.rows, w.pos, w.T);
-    attn_begin<KS>(s, x, seen);
+    attn_begin<KS>(s, x, a.l.head_size, seen);
   }
   const int least = attn_least(s.seen);
   const int most = -attn_least(-s.seen);
@@ -628,8 +619,8 @@ __global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs
       if (16 * d + 4 * g < l.head_size) attn_store(a, w, 16 * wave + row, 16 * d + 4 * g, s.o[d], s.M, s.sum, (float)s.E);
 }
 
-constexpr int kAttnBlocks = 512;        // workgroups that keep the card's 256 CUs busy
-constexpr int kAttnUnits = kAttnBlocks / 2;  // row tiles that are divided among workgroups, at most
+constexpr int kAttnBlocks = 512;  // workgroups that the keys of fewer row tiles are divided among: two for each CU
+constexpr int kAttnUnits = 256;   // row tiles that fill the card by themselves: one for each CU
 
 inline size_t attn_part(int head_size) { return 16 * ((head_size + 3) / 4 + 1); }  // bytes of a row's part
 
@@ -645,9 +636,15 @@ static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n
   p.many = pairs * ((rows + 63) / 64) >= kAttnBlocks / 2 && rows >= 64;
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
-  p.waves = p.many || c->head_size > 128 ? 4 : 8;
-  const long long most = (c->seq_len + 64LL * p.waves - 1) / (64 * p.waves);  // every wave has a tile to do
-  p.nsplit = p.many ? 1 : (int)max(1LL, min(most, min(64LL, kAttnBlocks / p.units)));
+  // Eight waves a workgroup where the tiles alone fill the card (sixteen ragged decode rows of 32 heads: 34.4 us, with four
+  // 35.1); else four, each alone on its SIMD until the card is full (one row of 32 heads over 2048 keys: 10.6 us, with
+  // eight 11.1), and keys divided until there are two workgroups for each CU (eight 32768-key rows of 8 K/V heads: 66 us,
+  // with one for each CU 73), but no further than each wave has a tile.  Tiles that fill the card are not divided (128 rows
+  // of 32 heads over 1152 keys: 13.8 us, in two 25).
+  const bool fills = p.units >= kAttnUnits;
+  p.waves = p.many || !fills || c->head_size > 128 ? 4 : 8;
+  const long long most = (c->seq_len + 64LL * p.waves - 1) / (64 * p.waves);
+  p.nsplit = p.many || fills ? 1 : (int)max(1LL, min(most, min(64LL, kAttnBlocks / p.units)));
   return p;
 }
 
@@ -658,7 +655,7 @@ static hipError_t attn_launch(const Q8AttnArgs& a, const AttnPlan& p, hipStream_
     hipLaunchKernelGGL((k_q8_attn_many<KS, KS <= 2 ? 4 : 2>), grid, block, 0, s, a);
     return hipGetLastError();
   }
-  const size_t lds = (size_t)p.waves * a.lrows * (64 * KS + 4 + 3) * sizeof(float);
+  const size_t lds = (size_t)p.waves * a.lrows * (64 * KS + 4 + 4) * sizeof(float);
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)k_q8_attn_few<KS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
