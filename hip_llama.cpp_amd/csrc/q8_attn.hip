@@ -11,7 +11,8 @@
 // value block's scale, w_t = 2^(x_t - m) sv_t, which is what has to be small beside the row's largest w: with
 // sv = f 2^e, 1/2 <= f < 1, the running maximum is taken of x_t + e_t, u_t = 2^(x_t + e_t - M) is at most 1 and
 // n_t = u_t f_t 0x7f7f7f.  The sum of the weights adds u_t 2^(E - e_t), E the largest e so far; value scales under
-// 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not.
+// 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not.  M is the maximum of
+// one step's 64 to 256 keys, so that a large weight elsewhere costs the step's own no digits; the steps are summed in fp32.
 //
 // One i8 product does 16x16x64 in the time in which fp32's does 16x16x8 on eight times the registers; the cache
 // is read as it is, without a conversion.
@@ -254,7 +255,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
         for (int i = 0; i < 4; ++i)
           if (64 * n + 4 * j + i >= left) x[n][j][i] = -INFINITY;
   }
-  float m = s.M;
+  float m = kNone;  // of this step alone: it sets the size that the step's weights are rounded to
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -262,8 +263,9 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = fmaxf(m, x[n][j][i]);
   m = rows_max(m);
-  const float alpha = __builtin_amdgcn_exp2f(s.M - m);
-  s.M = m;
+  const float M = fmaxf(s.M, m);
+  const float alpha = __builtin_amdgcn_exp2f(s.M - M), beta = __builtin_amdgcn_exp2f(m - M);
+  s.M = M;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -279,7 +281,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     if (edge && 64 * n >= left) continue;  // 0 x NaN of a block behind the row
     sum = fmaf(part, c.lift[n], sum);
   }
-  s.sum = fmaf(__builtin_ldexpf(s.sum, grow), alpha, sum);
+  s.sum = fmaf(__builtin_ldexpf(s.sum, grow), alpha, sum * beta);
   i4 p[NT][3];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -319,7 +321,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
         const i4(&r)[3] = acc[(u - 1) & 1];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          s.o[u - 1][i] = fmaf(s.o[u - 1][i], alpha, fmaf((float)r[2][i], 65536.f, (float)((r[1][i] << 8) + r[0][i])));
+          s.o[u - 1][i] = fmaf(fmaf((float)r[2][i], 65536.f, (float)((r[1][i] << 8) + r[0][i])), beta, s.o[u - 1][i] * alpha);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
