@@ -4,7 +4,7 @@
 //
 // Both products run on the int8 matrix cores with the cache's codes as they are, and still have fp32's accuracy.
 // The fp32 factor on the other side is held as a 24-bit integer n = d2 2^16 + d1 2^8 + d0 of three signed bytes
-// (balanced digits: the bytes of n + 0x808080, each less 128), so
+// (balanced digits: those of n + 0x8080, the lower two less 0x80), so
 //   sum n c = 2^16 sum d2 c + (2^8 sum d1 c + sum d0 c),
 // three exact int8 products with int32 sums.  For the scores n = q / 2^e 0x7f7f7f, with 2^e the power of two over a
 // row's largest |q|: off by 2^-24 of that, as an fp32 number is.  For the values it is the softmax weight times the
@@ -69,15 +69,13 @@ TL_DEVICE unsigned rows_umax(unsigned v) {
   return max(r.x, r.y);
 }
 
-// Balanced digits of four 24-bit integers (in the low bytes of t) as bytes 0 .. 3 of three words, lowest digit first.
-TL_DEVICE void digits4(const unsigned (&n)[4], int& p0, int& p1, int& p2) {
-  unsigned t[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) t[i] = (n[i] + 0x808080u) ^ 0x808080u;
+// The digits of four integers n, given t = n + 0x8080 with anything above its 24 bits, as bytes 0 .. 3 of three words,
+// lowest digit first: the added 0x80s carry, the low bytes less 0x80 are the two lower digits, the third is the top one.
+TL_DEVICE void digits4(const unsigned (&t)[4], int& p0, int& p1, int& p2) {
   const unsigned a = __builtin_amdgcn_perm(t[1], t[0], 0x05010400u), b = __builtin_amdgcn_perm(t[3], t[2], 0x05010400u);
   const unsigned c = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0602u), d = __builtin_amdgcn_perm(t[3], t[2], 0x06020c0cu);
-  p0 = (int)__builtin_amdgcn_perm(b, a, 0x05040100u);
-  p1 = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+  p0 = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+  p1 = (int)(__builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u);
   p2 = (int)(c | d);
 }
 
@@ -155,7 +153,7 @@ TL_DEVICE void attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
     for (int e = 0; e < 4; ++e) {
       unsigned n[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) n[c] = (unsigned)(int)rintf(__builtin_ldexpf(x[k][4 * e + c], -s.qe) * kDigits);
+      for (int c = 0; c < 4; ++c) n[c] = (unsigned)(int)rintf(__builtin_ldexpf(x[k][4 * e + c], -s.qe) * kDigits) + 0x8080u;
       int p0, p1, p2;
       digits4(n, p0, p1, p2);
       s.q[0][k][e] = p0;
@@ -289,7 +287,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     for (int j = 0; j < 4; ++j) {
       unsigned w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmaf(x[n][j][i], c.f[n], 8388608.f));  // low bytes: the nearest integer
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmaf(x[n][j][i], c.f[n], 8421504.f));  // 2^23 + 0x8080: low bytes n + 0x8080, rounded to nearest
       int p0, p1, p2;
       digits4(w, p0, p1, p2);
       p[n][0][j] = p0;
