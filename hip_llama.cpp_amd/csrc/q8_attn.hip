@@ -162,19 +162,18 @@ TL_DEVICE void attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
     }
 }
 
-// Scales of this lane's sixteen keys in each of NT tiles of 64 from t0 on; those of keys that nobody sees are 0.
+// Scales of this lane's sixteen keys in each of NT tiles of 64 from t0 on; behind the last key those of its block.
 template <int NT>
 struct AttnScales {
   float sk[NT], f[NT], lift[NT];
   int e[NT];
   TL_DEVICE void load(const Q8AttnArgs& a, const float* ks, const float* vs, int t0, int T) {
-    const int g = (threadIdx.x & 63) >> 4;
+    const unsigned g16 = threadIdx.x & 48u, last = (unsigned)(T - 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int t = t0 + 64 * n + 16 * g;
-      const int j = min(t, T - 1) >> a.l.block_log2;
-      sk[n] = t < T ? ks[j] : 0.f;
-      f[n] = t < T ? vs[j] : 0.f;
+      const unsigned j = min(t0 + 64u * n + g16, last) >> a.l.block_log2;
+      sk[n] = ks[j];
+      f[n] = vs[j];
     }
   }
 };
@@ -191,14 +190,14 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     c.e[n] = c.f[n] > 0.f ? __builtin_amdgcn_frexp_expf(c.f[n]) : -126;
     top = max(top, c.e[n]);
   }
-  {
+  if (__any(top > s.E)) {  // rare behind the first step
     v2u r = __builtin_amdgcn_permlane32_swap((unsigned)top, (unsigned)top, false, false);
     top = max((int)r.x, (int)r.y);
     r = __builtin_amdgcn_permlane16_swap((unsigned)top, (unsigned)top, false, false);
     top = max((int)r.x, (int)r.y);
+    s.sum = __builtin_ldexpf(s.sum, top - s.E);
+    s.E = top;
   }
-  const int grow = top - s.E;
-  s.E = top;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     c.e[n] = max(c.e[n], top - 40);
@@ -252,6 +251,9 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (64 * n + 4 * j + i >= left) x[n][j][i] = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      if (64 * n >= left) c.f[n] = c.lift[n] = 0.f;  // a block behind the row may hold NaN
   }
   float m = kNone;  // of this step alone: it sets the size that the step's weights are rounded to
 #pragma unroll
@@ -276,10 +278,9 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     float part = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) part += (x[n][j][0] + x[n][j][1]) + (x[n][j][2] + x[n][j][3]);
-    if (edge && 64 * n >= left) continue;  // 0 x NaN of a block behind the row
     sum = fmaf(part, c.lift[n], sum);
   }
-  s.sum = fmaf(__builtin_ldexpf(s.sum, grow), alpha, sum * beta);
+  s.sum = fmaf(s.sum, alpha, sum * beta);
   i4 p[NT][3];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -396,12 +397,12 @@ TL_DEVICE void attn_store(const Q8AttnArgs& a, const AttnUnit& w, int r, int d, 
   }
 }
 
-// 16 bytes a lane from memory to LDS, at `to` + 16 * lane; lds_wait: everybody's have arrived.  Written out, because
-// with the builtin the compiler waits for every load under way before the next read of any LDS.  m0 has no other use
-// in a kernel that calls this.
-TL_DEVICE void lds_bring(const int8_t* from, i4* to) {
+// 16 bytes a lane from memory, at `from` + the lane's offset, to LDS, at `to` + 16 * lane; lds_wait: everybody's have
+// arrived.  Written out, because with the builtin the compiler waits for every load under way before the next read of any
+// LDS.  m0 has no other use in a kernel that calls this.
+TL_DEVICE void lds_bring(const int8_t* from, unsigned offset, i4* to) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)to);
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(at) : "memory");
 }
 TL_DEVICE void lds_wait() {
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
 // chunk's keys while the values are.  LDS holds the codes in the order in which the lanes want them, one KiB for
 // each operand of a product, so that a load (16 bytes a lane, memory to LDS) and a read are both linear in the lane.
 template <int KS, int NT>
-__global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs a) {
+__global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp
   __shared__ __attribute__((aligned(1024))) i4 kbuf[NT * 4 * KS * 64];
   __shared__ __attribute__((aligned(1024))) i4 vbuf[NT * 4 * KS * 64];
@@ -566,14 +567,17 @@ __global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs
   const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
 
   // wave i brings operands i, i + 4, ...; tiles behind the last key are not brought
+  unsigned key_at[KS];
+#pragma unroll
+  for (int c = 0; c < KS; ++c)
+    key_at[c] = (16 * (row >> 2) + 4 * wave + (row & 3)) * l.lanes + (64 * c + 16 * g < l.lanes ? 64 * c + 16 * g : 0);
+  const unsigned value_at = g * 16 * l.lanes + 16 * row;
   auto keys_in = [&](int t0) {
 #pragma unroll
     for (int f = 0; f < NT * KS; ++f) {
-      const int n = f / KS, c = f % KS, j = wave;  // operand (n, j, c)
+      const int n = f / KS, c = f % KS;  // operand (n, wave, c)
       if (t0 + 64 * n >= w.T) continue;
-      const int d = 64 * c + 16 * g;
-      const int8_t* src = k + (long long)(t0 + 64 * n + 16 * (row >> 2) + 4 * j + (row & 3)) * l.lanes + (d < l.lanes ? d : 0);
-      lds_bring(src, &kbuf[((n * 4 + j) * KS + c) * 64]);
+      lds_bring(k + (long long)(t0 + 64 * n) * l.lanes, key_at[c], &kbuf[((n * 4 + wave) * KS + c) * 64]);
     }
   };
   auto values_in = [&](int t0) {
@@ -581,8 +585,7 @@ __global__ void __launch_bounds__(256, KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs
     for (int f = 0; f < NT * KS; ++f) {
       const int n = f / KS, d = (f % KS) * 4 + wave;  // operand (n, d)
       if (t0 + 64 * n >= w.T || 16 * d >= l.lanes) continue;
-      const int8_t* src = v + (long long)((t0 >> 4) + 4 * n + g) * (16 * l.lanes) + 256 * d + 16 * row;
-      lds_bring(src, &vbuf[(n * 4 * KS + d) * 64]);
+      lds_bring(v + (long long)(t0 + 64 * n) * l.lanes + 256 * d, value_at, &vbuf[(n * 4 * KS + d) * 64]);
     }
   };
 
@@ -652,7 +655,7 @@ template <int KS>
 static hipError_t attn_launch(const Q8AttnArgs& a, const AttnPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.units * p.nsplit)), block(64 * p.waves);
   if (p.many) {
-    hipLaunchKernelGGL((k_q8_attn_many<KS, KS <= 2 ? 4 : 2>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((k_q8_attn_many<KS, KS == 1 ? 4 : 2>), grid, block, 0, s, a);
     return hipGetLastError();
   }
   const size_t lds = (size_t)p.waves * a.lrows * (64 * KS + 4 + 4) * sizeof(float);

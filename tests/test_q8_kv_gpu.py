@@ -280,12 +280,12 @@ def test_attention(gpu, handle, case):
     dev.check("attention leaves the cache")
 
 
-@pytest.mark.parametrize("nt", [1, 40])
-def test_attention_values_of_very_different_size(gpu, handle, nt):
+@pytest.mark.parametrize("H,nt", [(2, 1), (2, 40), (90, 70)])
+def test_attention_values_of_very_different_size(gpu, handle, H, nt):
     """Value blocks a million times smaller than others keep their share where the large ones' weights vanish, and so
     do blocks of zeros in the sum of the weights."""
     r = rng(nt)
-    B, H, hs, S, block = 3, 2, 64, 600, 16
+    B, hs, S, block = 3, 64, 600, 16
     ref = Cache(B, 1, H, hs, S, block, r)
     k, v = rows(r, B, S, H, hs) * np.float32(0.2), rows(r, B, S, H, hs)
     v[:, 100:300] *= np.float32(1e-6)
@@ -299,8 +299,9 @@ def test_attention_values_of_very_different_size(gpu, handle, nt):
     dev = Device(gpu, handle, ref)
     pos = [S - nt] * B
     got = dev.attend(0, pos, None, q).reshape(q.shape)
-    want, bound = ref.attend(0, pos, [nt] * B, nt, q, 1)
-    hold(got, want, bound, "different sizes")
+    some = [0, nt - 1]
+    want, bound = ref.attend(0, pos, [nt] * B, nt, q, 1, some)
+    hold(got[:, some], want[:, some], bound[:, some], "different sizes")
     # That bound goes by the largest value, far above what the last row gets: hold it to its own size.  A weight times
     # its value block's scale, w_t = p_t sv_t, is held as n_t / 0x7f7f7f of 2^M with max w >= 2^M / 2, so it is off by
     # at most half a step, 2^M 2^-24 (1 + 2^-7) <= 2^-22 max w, times a code of at most 127; beside that each term is off by
@@ -349,17 +350,38 @@ def test_attention_sees_nothing_behind_its_position(gpu, handle, nt):
         np.testing.assert_array_equal(got[0, ~seen], before.reshape(got.shape)[0, ~seen])
 
 
-@pytest.mark.parametrize("nt", [1, 20])
-def test_attention_queries_not_finite(gpu, handle, nt):
+@pytest.mark.parametrize("B,H,mul", [(2, 2, 2), (64, 4, 4)])
+@pytest.mark.parametrize("hs", [48, 128])
+def test_attention_rows_before_a_bad_block(gpu, handle, B, H, mul, hs):
+    """A NaN block in the middle of what a row tile sees leaves the tile's earlier rows as they were."""
+    r = rng(B + hs)
+    S, block, nt, pos = 100, 16, 20, 40
+    ref, dev = filled(gpu, handle, r, B, 1, H, hs, S, block, [60] * B, 0)
+    q = r.standard_normal((B, nt, H * mul, hs)).astype(np.float32)
+    before = dev.attend(0, [pos] * B, None, q).reshape(B, nt, H, mul, hs)
+    for w in "kv":
+        kept = ref.scales[w].copy()
+        ref.scales[w][:, 0, 1, 3] = np.nan  # tokens 48 .. 63 of one head
+        dev.upload()
+        got = dev.attend(0, [pos] * B, None, q).reshape(before.shape)
+        assert np.isnan(got[:, 8:, 1]).all(), w
+        got[:, 8:, 1] = before[:, 8:, 1]
+        np.testing.assert_array_equal(got, before, w)
+        ref.scales[w][:] = kept
+
+
+@pytest.mark.parametrize("B,H,nt", [(2, 2, 1), (2, 2, 20), (64, 4, 20)])
+def test_attention_queries_not_finite(gpu, handle, B, H, nt):
     """A query with a NaN or an infinity has a NaN result; the rows beside it keep theirs."""
     r = rng(nt)
-    B, H, mul, hs, S = 2, 2, 4, 64, 200
-    ref, dev = filled(gpu, handle, r, B, 1, H, hs, S, 32, [150, 150], 0)
+    mul, hs, S = 4, 64, 200
+    ref, dev = filled(gpu, handle, r, B, 1, H, hs, S, 32, [150] * B, 0)
     q = r.standard_normal((B, nt, H * mul, hs)).astype(np.float32)
-    before = dev.attend(0, [100, 120], None, q).reshape(q.shape)
+    pos = [100 + 20 * (b & 1) for b in range(B)]
+    before = dev.attend(0, pos, None, q).reshape(q.shape)
     q[0, 0, 3, 5] = np.nan
     q[1, nt - 1, 6, 63] = np.inf
-    got = dev.attend(0, [100, 120], None, q).reshape(q.shape)
+    got = dev.attend(0, pos, None, q).reshape(q.shape)
     assert np.isnan(got[0, 0, 3]).all() and np.isnan(got[1, nt - 1, 6]).all()
     got[0, 0, 3], got[1, nt - 1, 6] = before[0, 0, 3], before[1, nt - 1, 6]
     np.testing.assert_array_equal(got, before)
