@@ -133,13 +133,15 @@ TL_DEVICE int attn_query(float (&x)[KS][16], const Q8AttnArgs& a, int b, int h, 
 template <int KS>
 TL_DEVICE void attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen) {
   s.seen = seen;
-  const int left = hs - 16 * ((threadIdx.x & 63) >> 4);
+  if (hs < 64 * KS) {
+    const int left = hs - 16 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (64 * k + e >= left) x[k][e] = 0.f;
+  }
   unsigned top = 0;
-#pragma unroll
-  for (int k = 0; k < KS; ++k)
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (64 * k + e >= left) x[k][e] = 0.f;
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -296,6 +298,11 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
       p[n][2][j] = p2;
     }
 
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.o[d][i] *= alpha;
+
   ready();
   // values, in the same turns
   {
@@ -320,7 +327,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
         const i4(&r)[3] = acc[(u - 1) & 1];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          s.o[u - 1][i] = fmaf(fmaf((float)r[2][i], 65536.f, (float)((r[1][i] << 8) + r[0][i])), beta, s.o[u - 1][i] * alpha);
+          s.o[u - 1][i] = fmaf(fmaf((float)r[2][i], 65536.f, (float)((r[1][i] << 8) + r[0][i])), beta, s.o[u - 1][i]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -381,21 +388,29 @@ TL_DEVICE void parts_join(const f4 (&x)[N], const f4 (&st)[N], int n, f4& o, flo
   E = top;
 }
 
-// Dimensions d .. d + 3 of row r of the unit, from its sums.  A row without keys is zeros.
-TL_DEVICE void attn_store(const Q8AttnArgs& a, const AttnUnit& w, int r, int d, f4 o, float M, float sum, float E) {
-  const int hs = a.l.head_size, i = (w.r0 + r) / a.mul;
-  float* dst = a.out + ((long long)w.b * a.call.n_tokens + i) * a.out_stride + (long long)(w.h * a.mul + w.r0 + r - i * a.mul) * hs + d;
-  const float inv = 1.f / (sum * kDigits);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = M == kNone && sum == 0.f ? 0.f : __builtin_ldexpf(o[e] * inv, (int)E);
-  if (a.vec) {
-    *reinterpret_cast<f4*>(dst) = o;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d + e < hs) dst[e] = o[e];
+// Where row r of the unit goes, and its sums' factor: 2^e inv.  A row without keys is zeros.
+struct AttnOut {
+  float* at;
+  float inv;
+  int e;
+  TL_DEVICE AttnOut(const Q8AttnArgs& a, const AttnUnit& w, int r, float M, float sum, float E) {
+    const int i = (w.r0 + r) / a.mul;
+    at = a.out + ((long long)w.b * a.call.n_tokens + i) * a.out_stride + (long long)(w.h * a.mul + w.r0 + r - i * a.mul) * a.l.head_size;
+    inv = M == kNone && sum == 0.f ? 0.f : 1.f / (sum * kDigits);
+    e = (int)E;
   }
-}
+  TL_DEVICE void store(const Q8AttnArgs& a, int d, f4 o) const {  // dimensions d .. d + 3
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = __builtin_ldexpf(o[c] * inv, e);
+    if (a.vec) {
+      *reinterpret_cast<f4*>(at + d) = o;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (d + c < a.l.head_size) at[d + c] = o[c];
+    }
+  }
+};
 
 // 16 bytes a lane from memory, at `from` + the lane's offset, to LDS, at `to` + 16 * lane; lds_wait: everybody's have
 // arrived.  Written out, because with the builtin the compiler waits for every load under way before the next read of any
@@ -508,7 +523,7 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
     float M = kNone, E = -126.f, sum = 0.f;
     parts_join(x, st, waves, o, M, sum, E);
     if (a.nsplit == 1) {
-      attn_store(a, w, r, 4 * d, o, M, sum, E);
+      AttnOut(a, w, r, M, sum, E).store(a, 4 * d, o);
       continue;
     }
     const unsigned at = mine + (split * a.lrows + r) * part;
@@ -542,7 +557,7 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
       }
       parts_join(x, st, a.nsplit - n0, o, M, sum, E);
     }
-    attn_store(a, w, r, 4 * d, o, M, sum, E);
+    AttnOut(a, w, r, M, sum, E).store(a, 4 * d, o);
   }
 }
 
@@ -616,10 +631,11 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
                       [&](int n, int d) { return vbuf[(n * 4 * KS + d) * 64 + lane]; }, ready);
   }
   s.sum = rows_sum(s.sum);
-  if (16 * wave + row < w.nr)
+  if (16 * wave + row >= w.nr) return;
+  const AttnOut out(a, w, 16 * wave + row, s.M, s.sum, (float)s.E);
 #pragma unroll
-    for (int d = 0; d < 4 * KS; ++d)
-      if (16 * d + 4 * g < l.head_size) attn_store(a, w, 16 * wave + row, 16 * d + 4 * g, s.o[d], s.M, s.sum, (float)s.E);
+  for (int d = 0; d < 4 * KS; ++d)
+    if (16 * d + 4 * g < l.head_size) out.store(a, 16 * d + 4 * g, s.o[d]);
 }
 
 constexpr int kAttnBlocks = 512;  // workgroups that the keys of fewer row tiles are divided among: two for each CU
