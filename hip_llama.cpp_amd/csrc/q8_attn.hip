@@ -23,6 +23,7 @@
 // and the four steps together the sixteen bytes that the value product's second operand wants from that lane; the
 // cache's value layout (16 tokens of a dimension side by side) is its first operand.  Nothing crosses lanes but
 // the row maximum.
+#include <type_traits>
 #include "q8_kv.hpp"
 
 namespace tl {
@@ -31,7 +32,6 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
 constexpr float kNone = -1e30f;       // a maximum over nothing
-constexpr int kWaves = 8;             // of a workgroup, at most
 
 struct Q8AttnArgs {
   Q8KVLayer l;
@@ -336,8 +336,10 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
 
 // The least number of keys that one of the wave's rows sees.
 TL_DEVICE int attn_least(int seen) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) seen = min(seen, __shfl_xor(seen, o, 64));
+  seen = min(seen, __builtin_amdgcn_mov_dpp(seen, 0xB1, 0xF, 0xF, false));   // common.hpp row16_max's steps
+  seen = min(seen, __builtin_amdgcn_mov_dpp(seen, 0x4E, 0xF, 0xF, false));
+  seen = min(seen, __builtin_amdgcn_mov_dpp(seen, 0x141, 0xF, 0xF, false));
+  seen = min(seen, __builtin_amdgcn_mov_dpp(seen, 0x140, 0xF, 0xF, false));
   return __builtin_amdgcn_readfirstlane(seen);
 }
 
@@ -466,12 +468,15 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
   if (!attn_unit(a, unit % pairs, a.tiles - 1 - unit / pairs, 16, w)) return;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  // few keys for so many workgroups: as many as have a tile for each wave, or one alone for up to two each
+  const int tiles = (w.T + 63) / 64, nsplit = tiles <= 2 * waves ? 1 : min(a.nsplit, (tiles + waves - 1) / waves);
+  if (split >= nsplit) return;
   const int8_t* k = l.k + w.b * l.seq_codes + w.h * l.head_codes;
   const int8_t* v = l.v + w.b * l.seq_codes + w.h * l.head_codes;
   const float* ks = l.ks + w.b * l.seq_scales + w.h * l.head_scales;
   const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
   const int row = lane & 15, g = lane >> 4;
-  const int step = 64 * waves * a.nsplit;
+  const int step = 64 * waves * nsplit;
   int t0 = 64 * (split * waves + wave);
   AttnRows<KS> s;
   s.none();
@@ -512,17 +517,21 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
   const unsigned mine = unit * a.nsplit * a.lrows * part;  // of the unit's first
   for (int it = threadIdx.x; it < w.nr * quads; it += blockDim.x) {
     const int r = it / quads, d = it - r * quads;
-    f4 x[kWaves], st[kWaves];
-#pragma unroll
-    for (int n = 0; n < kWaves; ++n) {
-      const int at = min(n, waves - 1) * a.lrows + r;
-      st[n] = stat[at];
-      x[n] = *reinterpret_cast<const f4*>(lds + at * wide + 4 * d);
-    }
     f4 o = {0.f, 0.f, 0.f, 0.f};
     float M = kNone, E = -126.f, sum = 0.f;
-    parts_join(x, st, waves, o, M, sum, E);
-    if (a.nsplit == 1) {
+    auto join = [&](auto count) {
+      constexpr int N = decltype(count)::value;
+      f4 x[N], st[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        st[n] = stat[n * a.lrows + r];
+        x[n] = *reinterpret_cast<const f4*>(lds + (n * a.lrows + r) * wide + 4 * d);
+      }
+      parts_join(x, st, N, o, M, sum, E);
+    };
+    if (KS > 2 || waves == 4) join(std::integral_constant<int, 4>());
+    else join(std::integral_constant<int, 8>());
+    if (nsplit == 1) {
       AttnOut(a, w, r, M, sum, E).store(a, 4 * d, o);
       continue;
     }
@@ -530,14 +539,14 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
     st4_sc1(parts, at + 16 * d, o);
     if (d == 0) st4_sc1(parts, at + 16 * quads, f4{M, sum, E, 0.f});
   }
-  if (a.nsplit == 1) return;
+  if (nsplit == 1) return;
 
   // Parts are written through and read past the caches of the XCDs (sc1); each wave's have arrived before the count.
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
   if (threadIdx.x == 0) {
     const unsigned before = __hip_atomic_fetch_add(&a.arrived[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = before == (unsigned)a.nsplit - 1;
+    last = before == (unsigned)nsplit - 1;
     if (last) __hip_atomic_store(&a.arrived[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
@@ -547,15 +556,15 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
     const unsigned at = mine + r * part, stride = a.lrows * part;
     f4 o = {0.f, 0.f, 0.f, 0.f};
     float M = kNone, E = -126.f, sum = 0.f;
-    for (int n0 = 0; n0 < a.nsplit; n0 += 8) {  // eight parts under way at once, each joined to what is before it
+    for (int n0 = 0; n0 < nsplit; n0 += 8) {  // eight parts under way at once, each joined to what is before it
       f4 x[8], st[8];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const unsigned p = at + min(n0 + n, a.nsplit - 1) * stride;
+        const unsigned p = at + min(n0 + n, nsplit - 1) * stride;
         st[n] = ld4_sc1(parts, p + 16 * quads);
         x[n] = ld4_sc1(parts, p + 16 * d);
       }
-      parts_join(x, st, a.nsplit - n0, o, M, sum, E);
+      parts_join(x, st, nsplit - n0, o, M, sum, E);
     }
     AttnOut(a, w, r, M, sum, E).store(a, 4 * d, o);
   }
