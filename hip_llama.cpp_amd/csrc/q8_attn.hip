@@ -23,7 +23,6 @@
 // and the four steps together the sixteen bytes that the value product's second operand wants from that lane; the
 // cache's value layout (16 tokens of a dimension side by side) is its first operand.  Nothing crosses lanes but
 // the row maximum.
-#include <type_traits>
 #include "q8_kv.hpp"
 
 namespace tl {
@@ -32,6 +31,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
 constexpr float kNone = -1e30f;       // a maximum over nothing
+constexpr int kWaves = 4;             // of a workgroup
 
 struct Q8AttnArgs {
   Q8KVLayer l;
@@ -456,7 +456,7 @@ struct AttnTile {
 // its next values when the sums are.  The waves' results are joined in LDS; where several workgroups share a row tile, each leaves its result in the workspace and the last
 // one to arrive joins them, in the order of the splits whoever it is.
 template <int KS>
-__global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a) {
+__global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_few(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
   extern __shared__ __attribute__((aligned(16))) float lds[];
   __shared__ int last;
@@ -467,17 +467,17 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
   AttnUnit w;
   if (!attn_unit(a, unit % pairs, a.tiles - 1 - unit / pairs, 16, w)) return;
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // few keys for so many workgroups: as many as have a tile for each wave, or one alone for up to two each
-  const int tiles = (w.T + 63) / 64, nsplit = tiles <= 2 * waves ? 1 : min(a.nsplit, (tiles + waves - 1) / waves);
+  const int tiles = (w.T + 63) / 64, nsplit = tiles <= 2 * kWaves ? 1 : min(a.nsplit, (tiles + kWaves - 1) / kWaves);
   if (split >= nsplit) return;
   const int8_t* k = l.k + w.b * l.seq_codes + w.h * l.head_codes;
   const int8_t* v = l.v + w.b * l.seq_codes + w.h * l.head_codes;
   const float* ks = l.ks + w.b * l.seq_scales + w.h * l.head_scales;
   const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
   const int row = lane & 15, g = lane >> 4;
-  const int step = 64 * waves * nsplit;
-  int t0 = 64 * (split * waves + wave);
+  const int step = 64 * kWaves * nsplit;
+  int t0 = 64 * (split * kWaves + wave);
   AttnRows<KS> s;
   s.none();
   if (t0 < w.T) {
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
 
   // join the waves' rows
   const int hs = l.head_size, wide = 64 * KS + 4;
-  f4* stat = reinterpret_cast<f4*>(lds + waves * a.lrows * wide);
+  f4* stat = reinterpret_cast<f4*>(lds + kWaves * a.lrows * wide);
   s.sum = rows_sum(s.sum);
   if (row < w.nr) {
     float* dst = lds + (wave * a.lrows + row) * wide + 4 * g;
@@ -519,18 +519,13 @@ __global__ void __launch_bounds__(KS < 3 ? 512 : 256) k_q8_attn_few(Q8AttnArgs a
     const int r = it / quads, d = it - r * quads;
     f4 o = {0.f, 0.f, 0.f, 0.f};
     float M = kNone, E = -126.f, sum = 0.f;
-    auto join = [&](auto count) {
-      constexpr int N = decltype(count)::value;
-      f4 x[N], st[N];
+    f4 x[kWaves], st[kWaves];
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        st[n] = stat[n * a.lrows + r];
-        x[n] = *reinterpret_cast<const f4*>(lds + (n * a.lrows + r) * wide + 4 * d);
-      }
-      parts_join(x, st, N, o, M, sum, E);
-    };
-    if (KS > 2 || waves == 4) join(std::integral_constant<int, 4>());
-    else join(std::integral_constant<int, 8>());
+    for (int n = 0; n < kWaves; ++n) {
+      st[n] = stat[n * a.lrows + r];
+      x[n] = *reinterpret_cast<const f4*>(lds + (n * a.lrows + r) * wide + 4 * d);
+    }
+    parts_join(x, st, kWaves, o, M, sum, E);
     if (nsplit == 1) {
       AttnOut(a, w, r, M, sum, E).store(a, 4 * d, o);
       continue;
@@ -647,43 +642,40 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
     if (16 * d + 4 * g < l.head_size) out.store(a, 16 * d + 4 * g, s.o[d]);
 }
 
-constexpr int kAttnBlocks = 512;  // workgroups that the keys of fewer row tiles are divided among: two for each CU
-constexpr int kAttnUnits = 256;   // row tiles that fill the card by themselves: one for each CU
+constexpr int kAttnUnits = 256;  // row tiles that fill the card by themselves: one for each CU
+constexpr int kMaxSplit = 128;
 
 inline size_t attn_part(int head_size) { return 16 * ((head_size + 3) / 4 + 1); }  // bytes of a row's part
 
 // How a call's rows and keys are divided.
 struct AttnPlan {
   bool many;
-  int waves, nsplit;
+  int nsplit;
   long long tiles, units;
 };
 static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads) {
   AttnPlan p;
   const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads), pairs = (long long)n_batches * c->n_kv_heads;
-  p.many = pairs * ((rows + 63) / 64) >= kAttnBlocks / 2 && rows >= 64;
+  p.many = pairs * ((rows + 63) / 64) >= kAttnUnits && rows >= 64;
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
-  // Eight waves a workgroup where the tiles alone fill the card (sixteen ragged decode rows of 32 heads: 34.4 us, with four
-  // 35.1); else four, each alone on its SIMD until the card is full (one row of 32 heads over 2048 keys: 10.6 us, with
-  // eight 11.1), and keys divided until there are two workgroups for each CU (eight 32768-key rows of 8 K/V heads: 66 us,
-  // with one for each CU 73), but no further than each wave has a tile.  Tiles that fill the card are not divided (128 rows
-  // of 32 heads over 1152 keys: 13.8 us, in two 25).
-  const bool fills = p.units >= kAttnUnits;
-  p.waves = p.many || !fills || c->head_size > 128 ? 4 : 8;
-  const long long most = (c->seq_len + 64LL * p.waves - 1) / (64 * p.waves);
-  p.nsplit = p.many || fills ? 1 : (int)max(1LL, min(most, min(64LL, kAttnBlocks / p.units)));
+  // The keys of few tiles are divided until there is a workgroup for each CU, but no further than each wave has a tile (one
+  // row of 32 heads over 2048 keys: 10.4 us; 16 rows: 13.8, with two for each CU 17), or two for each CU where each
+  // wave still has eight (eight 32768-key rows of 8 K/V heads: 66 us, with one 73).
+  const long long most = (c->seq_len + 64LL * kWaves - 1) / (64 * kWaves);
+  p.nsplit = p.many ? 1 : (int)max(1LL, min(most, min((long long)kMaxSplit, kAttnUnits / p.units)));
+  if (p.nsplit > 1 && most >= 16 * p.nsplit) p.nsplit = min(2 * p.nsplit, kMaxSplit);
   return p;
 }
 
 template <int KS>
 static hipError_t attn_launch(const Q8AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.units * p.nsplit)), block(64 * p.waves);
+  const dim3 grid((unsigned)(p.units * p.nsplit)), block(64 * kWaves);
   if (p.many) {
     hipLaunchKernelGGL((k_q8_attn_many<KS, KS == 1 ? 4 : 2>), grid, block, 0, s, a);
     return hipGetLastError();
   }
-  const size_t lds = (size_t)p.waves * a.lrows * (64 * KS + 4 + 4) * sizeof(float);
+  const size_t lds = (size_t)kWaves * a.lrows * (64 * KS + 4 + 4) * sizeof(float);
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)k_q8_attn_few<KS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
@@ -703,7 +695,7 @@ extern "C" size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batche
       !tl::q8kv_supported(c->head_size, c->block) || !attn_sizes_ok(c, n_heads))
     return 0;
   // a call of fewer rows may divide its keys among more workgroups, but never has more than this many parts
-  return tl::kAttnUnits * sizeof(unsigned) + (size_t)tl::kAttnBlocks * 16 * tl::attn_part(c->head_size);
+  return tl::kAttnUnits * sizeof(unsigned) + (size_t)2 * tl::kAttnUnits * 16 * tl::attn_part(c->head_size);
 }
 
 extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, const Q8KVCache* c, int layer,
