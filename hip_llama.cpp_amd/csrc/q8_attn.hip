@@ -656,7 +656,10 @@ struct AttnPlan {
 static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads) {
   AttnPlan p;
   const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads), pairs = (long long)n_batches * c->n_kv_heads;
-  p.many = pairs * ((rows + 63) / 64) >= kAttnUnits && rows >= 64;
+  // Tiles of 64 rows that fill the card go to k_q8_attn_many: from 256 of them on (256, of 32 heads x 512 rows: 16.5 us,
+  // k_q8_attn_few 19.1; 224: 15.1 and 16.1; 352: 22.4 and 28.6), at heads of up to 64, where the few rows' kernel fits four waves on a SIMD,
+  // from 512 (264, of 12 heads x 1400 rows: 24.0 us and 17.4; 564: 47.1 and 49.5).
+  p.many = rows >= 64 && pairs * ((rows + 63) / 64) >= (c->head_size <= 64 ? 2 : 1) * kAttnUnits;
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
   // The keys of few tiles are divided until there is a workgroup for each CU, but no further than each wave has a tile (one

@@ -242,6 +242,7 @@ ATTENDS = [  # B, L, H, mul, hs, S, block, pos, n, n_tokens, pad, shift
 ] + [  # rows enough to fill the card: a few hundred tiles of 64
     (16, 1, 16, 1, 64, 200, 32, [7 * b for b in range(16)], [66 - 4 * b for b in range(16)], 66, 0, 0),
     (32, 2, 4, 3, 48, 700, 16, [20 * b for b in range(32)], None, 30, 0, 0),
+    (64, 1, 4, 3, 48, 700, 16, [10 * b for b in range(64)], [30 - b % 9 for b in range(64)], 30, 4, 4),
     (64, 1, 2, 8, 128, 300, 64, [4 * b for b in range(64)], [b % 18 for b in range(64)], 17, 0, 0),
     (32, 1, 8, 5, 130, 350, 128, [9 * b for b in range(32)], None, 13, 2, 1),
     (64, 1, 4, 1, 200, 330, 32, [260, 3] * 32, [70, 65] * 32, 70, 4, 4),
@@ -280,7 +281,7 @@ def test_attention(gpu, handle, case):
     dev.check("attention leaves the cache")
 
 
-@pytest.mark.parametrize("H,nt", [(2, 1), (2, 40), (90, 70)])
+@pytest.mark.parametrize("H,nt", [(2, 1), (2, 40), (90, 70)])  # the last fills the card
 def test_attention_values_of_very_different_size(gpu, handle, H, nt):
     """Value blocks a million times smaller than others keep their share where the large ones' weights vanish, and so
     do blocks of zeros in the sum of the weights."""
@@ -370,7 +371,7 @@ def test_attention_rows_before_a_bad_block(gpu, handle, B, H, mul, hs):
         ref.scales[w][:] = kept
 
 
-@pytest.mark.parametrize("B,H,nt", [(2, 2, 1), (2, 2, 20), (64, 4, 20)])
+@pytest.mark.parametrize("B,H,nt", [(2, 2, 1), (2, 2, 20), (64, 4, 20)])  # the last fills the card
 def test_attention_queries_not_finite(gpu, handle, B, H, nt):
     """A query with a NaN or an infinity has a NaN result; the rows beside it keep theirs."""
     r = rng(nt)
