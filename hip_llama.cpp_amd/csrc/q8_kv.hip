@@ -1,9 +1,9 @@
 // q8_kv.hip — the int8 K/V cache: rows quantised as they are written, and read back
 // (include/thaDNN/thaDNN_q8_kv.hpp).
 //
-// Both kernels give a thread four dimensions of sixteen tokens: a float4 of each row, a dword of each key's
-// codes, and the four 16-byte runs in which the value codes of those dimensions lie side by side, so neither
-// layout needs an exchange between lanes.
+// Both kernels give a thread four dimensions of sixteen or eight tokens: a float4 of each row, a dword of each key's
+// codes, and the four runs in which the value codes of those dimensions lie side by side, so neither layout needs
+// an exchange between lanes.
 #include "q8_kv.hpp"
 
 using tl::f4;
@@ -41,7 +41,7 @@ namespace tl {
 
 // Dimensions d .. d + 3 of a row; those from head_size on read as 0.  A call passes over its rows once: nontemporal, which
 // is what carries the large calls (8 x 2048 rows of 4096 and their codes, MI355X: stored in 157 us without, 120 with, read
-// back in 134 and 129; one row each of sixteen sequences' blocks read back in 8.2 and 6.2).
+// back in 134 and 129 by 16 tokens a thread; one row each of sixteen sequences' blocks read back in 8.2 and 6.2).
 template <bool VEC>
 TL_DEVICE f4 row4_load(const float* row, int d, int head_size) {
   if constexpr (VEC) return __builtin_nontemporal_load(reinterpret_cast<const f4*>(row + d));
@@ -62,6 +62,7 @@ TL_DEVICE void row4_store(float* row, int d, int head_size, f4 x) {
   }
 }
 
+typedef int i2 __attribute__((ext_vector_type(2)));
 typedef int i4 __attribute__((ext_vector_type(4)));
 
 TL_DEVICE int byte_of(int x, int i) { return (int)(signed char)(x >> (8 * i)); }
@@ -259,12 +260,13 @@ struct LoadArgs {
   Q8KVCall call;
   float* x[2];
   long long stride;
-  int groups;   // groups of 16 slots that n_tokens rows may touch
+  int groups;   // groups of 8 slots that n_tokens rows may touch
   int columns;  // workgroups across a row
   int from;     // 0: keys and values, or keys alone; 1: values alone
 };
 
-// Thread: dimensions d .. d + 3 of one head in the 16 tokens of one group of slots.
+// Thread: dimensions d .. d + 3 of one head in the 8 tokens of one group of slots (8 x 2048 rows of 4096, MI355X: 117 us,
+// with 16 tokens 140, with 4 121).
 template <bool VEC>
 __global__ void __launch_bounds__(256) k_q8kv_load(LoadArgs a, int both) {
   keep_implicit_args();  // common.hpp
@@ -275,41 +277,38 @@ __global__ void __launch_bounds__(256) k_q8kv_load(LoadArgs a, int both) {
   const int jg = u % a.groups;
   u /= a.groups;
   const int which = both ? (int)(u & 1) : a.from, b = both ? u >> 1 : u;
-
   long long row0;
   int first, last;
   q8kv_span(a.call, l.seq_len, b, row0, first, last);
-  const int t0 = ((first >> 4) + jg) << 4;
+  const int t0 = ((first >> 3) + jg) << 3;
   if (first >= last || t0 >= last) return;
   const int quads = l.lanes / 4;
   const int at = col * 256 + threadIdx.x;
   const int h = at / quads, d = (at - h * quads) * 4;
   if (h >= l.heads || d >= l.head_size) return;
-
   const float scale = (which ? l.vs : l.ks)[b * l.seq_scales + h * l.head_scales + (t0 >> l.block_log2)];
-  const long long head = b * l.seq_codes + h * l.head_codes + (long long)t0 * l.lanes;
   float* dst = a.x[which] + ((long long)b * a.call.n_tokens + (t0 - row0)) * a.stride + (long long)h * l.head_size;
-  int w[16];  // keys: a dword of each token; values: four dwords of each dimension
+  int w[8];
   if (which == 0) {
-    const int* src = reinterpret_cast<const int*>(l.k + head + d);
+    const int* src = reinterpret_cast<const int*>(l.k + b * l.seq_codes + h * l.head_codes + (long long)t0 * l.lanes + d);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = t0 + i >= first && t0 + i < last ? src[(long long)i * (l.lanes / 4)] : 0;
+    for (int i = 0; i < 8; ++i) w[i] = src[(long long)i * (l.lanes / 4)];
   } else {
-    const i4* src = reinterpret_cast<const i4*>(l.v + head + d * 16);
+    const int8_t* src = l.v + b * l.seq_codes + h * l.head_codes + (long long)(t0 & ~15) * l.lanes + (t0 & 8) + d * 16;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const i4 q = src[e];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[4 * e + i] = q[i];
+      const i2 q = *reinterpret_cast<const i2*>(src + 16 * e);
+      w[2 * e] = q.x;
+      w[2 * e + 1] = q.y;
     }
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 8; ++i) {
     if (t0 + i < first || t0 + i >= last) continue;
     f4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      x[e] = __fmul_rn((float)(which == 0 ? byte_of(w[i], e) : byte_of(w[4 * e + i / 4], i % 4)), scale);
+      x[e] = __fmul_rn((float)(which == 0 ? byte_of(w[i], e) : byte_of(w[2 * e + i / 4], i % 4)), scale);
     row4_store<VEC>(dst + i * a.stride, d, l.head_size, x);
   }
 }
@@ -358,7 +357,7 @@ extern "C" thablasStatus_t thaDNN_q8_kv_load_batch(thablasHandle_t* handle, cons
   a.x[1] = v;
   a.stride = kv_stride;
   a.from = k ? 0 : 1;
-  const long long groups = ((long long)n_tokens + 14) / 16 + 1, most = ((long long)c->seq_len + 15) / 16;
+  const long long groups = ((long long)n_tokens + 6) / 8 + 1, most = ((long long)c->seq_len + 7) / 8;
   a.groups = (int)(groups < most ? groups : most);
   const long long columns = ((long long)c->n_kv_heads * (a.l.lanes / 4) + 255) / 256;
   a.columns = (int)columns;
