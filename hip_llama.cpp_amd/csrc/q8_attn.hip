@@ -32,6 +32,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
 constexpr float kNone = -1e30f;       // a maximum over nothing
 constexpr int kWaves = 4;             // of a workgroup
+constexpr int kCountStep = 32;        // a cache line for each count of arrivals
 
 struct Q8AttnArgs {
   Q8KVLayer l;
@@ -540,9 +541,9 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
   if (threadIdx.x == 0) {
-    const unsigned before = __hip_atomic_fetch_add(&a.arrived[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned before = __hip_atomic_fetch_add(&a.arrived[unit * kCountStep], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last = before == (unsigned)nsplit - 1;
-    if (last) __hip_atomic_store(&a.arrived[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (last) __hip_atomic_store(&a.arrived[unit * kCountStep], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!last) return;
@@ -698,7 +699,7 @@ extern "C" size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batche
       !tl::q8kv_supported(c->head_size, c->block) || !attn_sizes_ok(c, n_heads))
     return 0;
   // a call of fewer rows may divide its keys among more workgroups, but never has more than this many parts
-  return tl::kAttnUnits * sizeof(unsigned) + (size_t)2 * tl::kAttnUnits * 16 * tl::attn_part(c->head_size);
+  return tl::kAttnUnits * tl::kCountStep * sizeof(unsigned) + (size_t)2 * tl::kAttnUnits * 16 * tl::attn_part(c->head_size);
 }
 
 extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, const Q8KVCache* c, int layer,
@@ -717,13 +718,13 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   const tl::AttnPlan p = tl::attn_plan(c, n_batches, n_tokens, n_heads);
   if ((long long)n_tokens * mul > 0x7fffffffLL - 64 || p.units * p.nsplit > 0x7fffffffLL / 16) return THABLAS_STATUS_NOT_SUPPORTED;
   const int lrows = (int)min((long long)n_tokens * mul, 16LL);
-  const size_t need = p.nsplit > 1 ? tl::kAttnUnits * sizeof(unsigned) + (size_t)p.units * p.nsplit * lrows * tl::attn_part(c->head_size) : 0;
+  const size_t need = p.nsplit > 1 ? tl::kAttnUnits * tl::kCountStep * sizeof(unsigned) + (size_t)p.units * p.nsplit * lrows * tl::attn_part(c->head_size) : 0;
   if (need && (!work || ((uintptr_t)work & 15) || work_bytes < need)) return THABLAS_STATUS_INVALID_VALUE;
   a.call = {pos_d, n_d, n_batches, n_tokens};
   a.q = q;
   a.out = out;
   a.arrived = static_cast<unsigned*>(work);
-  a.part = reinterpret_cast<float*>(a.arrived + tl::kAttnUnits);
+  a.part = reinterpret_cast<float*>(a.arrived + tl::kAttnUnits * tl::kCountStep);
   a.q_stride = q_stride;
   a.out_stride = out_stride;
   a.n_heads = n_heads;
