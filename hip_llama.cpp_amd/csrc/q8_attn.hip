@@ -30,7 +30,7 @@ namespace tl {
 typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
-constexpr float kNone = -1e30f;       // a maximum over nothing
+constexpr float kNone = -3.4e38f;     // a maximum over nothing
 constexpr int kWaves = 4;             // of a workgroup
 constexpr int kCountStep = 32;        // a cache line for each count of arrivals
 
@@ -187,7 +187,7 @@ template <int KS, int NT, class Key, class Val, class Ready>
 TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
   constexpr int DT = 4 * KS;
   const int g = (threadIdx.x & 63) >> 4;
-  int top = s.E;
+  int top = s.E, grow = 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     c.e[n] = c.f[n] > 0.f ? __builtin_amdgcn_frexp_expf(c.f[n]) : -126;
@@ -198,7 +198,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     top = max((int)r.x, (int)r.y);
     r = __builtin_amdgcn_permlane16_swap((unsigned)top, (unsigned)top, false, false);
     top = max((int)r.x, (int)r.y);
-    s.sum = __builtin_ldexpf(s.sum, top - s.E);
+    grow = top - s.E;
     s.E = top;
   }
 #pragma unroll
@@ -268,6 +268,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
   m = rows_max(m);
   const float M = fmaxf(s.M, m);
   const float alpha = __builtin_amdgcn_exp2f(s.M - M), beta = __builtin_amdgcn_exp2f(m - M);
+  s.sum = s.sum == 0.f ? 0.f : s.sum * __builtin_amdgcn_exp2f((s.M - M) + (float)grow);  // either alone may be out of range
   s.M = M;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -283,7 +284,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     for (int j = 0; j < 4; ++j) part += (x[n][j][0] + x[n][j][1]) + (x[n][j][2] + x[n][j][3]);
     sum = fmaf(part, c.lift[n], sum);
   }
-  s.sum = fmaf(s.sum, alpha, sum * beta);
+  s.sum = fmaf(sum, beta, s.sum);
   i4 p[NT][3];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -454,8 +455,8 @@ struct AttnTile {
 
 // Few rows: one workgroup takes 16 query rows of one (sequence, K/V head) and, of their keys, every nsplit-th run of
 // a 64-key tile for each of its waves.  A wave asks for its next keys as soon as the scores are done with these, and for
-// its next values when the sums are.  The waves' results are joined in LDS; where several workgroups share a row tile, each leaves its result in the workspace and the last
-// one to arrive joins them, in the order of the splits whoever it is.
+// its next values when the sums are.  The waves' results are joined in LDS; where several workgroups share a row tile,
+// each leaves its result in the workspace and the last one to arrive joins them, in the order of the splits whoever it is.
 template <int KS>
 __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_few(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
@@ -658,8 +659,8 @@ static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n
   AttnPlan p;
   const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads), pairs = (long long)n_batches * c->n_kv_heads;
   // Tiles of 64 rows that fill the card go to k_q8_attn_many: from 256 of them on (256, of 32 heads x 512 rows: 16.5 us,
-  // k_q8_attn_few 19.1; 224: 15.1 and 16.1; 352: 22.4 and 28.6), at heads of up to 64, where the few rows' kernel fits four waves on a SIMD,
-  // from 512 (264, of 12 heads x 1400 rows: 24.0 us and 17.4; 564: 47.1 and 49.5).
+  // k_q8_attn_few 19.1; 224: 15.1 and 16.1; 352: 22.4 and 28.6), at heads of up to 64, where the few rows' kernel fits
+  // four waves on a SIMD, from 512 (264, of 12 heads x 1400 rows: 24.0 us and 17.4; 564: 47.1 and 49.5).
   p.many = rows >= 64 && pairs * ((rows + 63) / 64) >= (c->head_size <= 64 ? 2 : 1) * kAttnUnits;
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
@@ -695,7 +696,7 @@ static bool attn_sizes_ok(const Q8KVCache* c, int n_heads) {
 }
 
 extern "C" size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads) {
-  if (!c || n_batches <= 0 || n_tokens <= 0 || !tl::q8kv_sizes_ok(c->n_batches, c->n_layers, c->n_kv_heads, c->head_size, c->seq_len) ||
+  if (!c || n_batches <= 0 || n_batches > c->n_batches || n_tokens <= 0 || !tl::q8kv_sizes_ok(c->n_batches, c->n_layers, c->n_kv_heads, c->head_size, c->seq_len) ||
       !tl::q8kv_supported(c->head_size, c->block) || !attn_sizes_ok(c, n_heads))
     return 0;
   // a call of fewer rows may divide its keys among more workgroups, but never has more than this many parts

@@ -7,6 +7,7 @@
 namespace tl {
 
 constexpr int kQ8KVMaxHead = 256;
+constexpr int kQ8KVMaxSeq = 1 << 30;
 
 // One layer of the cache as a kernel sees it.
 struct Q8KVLayer {
@@ -50,8 +51,8 @@ inline long long q8kv_slots(int seq_len, int block) {
   return ((long long)seq_len + unit - 1) / unit * unit;
 }
 inline bool q8kv_sizes_ok(int n_batches, int n_layers, int n_kv_heads, int head_size, int seq_len) {
-  // a row of K/V fits an int, and so does every slot
-  return n_batches > 0 && n_layers > 0 && n_kv_heads > 0 && head_size > 0 && seq_len > 0 && seq_len <= 0x7fffff00 &&
+  // a row of K/V fits an int, and so does every slot with a stride over all waves of a call
+  return n_batches > 0 && n_layers > 0 && n_kv_heads > 0 && head_size > 0 && seq_len > 0 && seq_len <= kQ8KVMaxSeq &&
          (long long)n_kv_heads * head_size <= 0x7fffffffLL;
 }
 inline size_t q8kv_part(unsigned __int128 bytes) {  // a part of the cache's allocation; too large: 0
@@ -107,10 +108,15 @@ struct Q8KVDevice {
   bool ok = true;
   explicit Q8KVDevice(int dev) {
     int cur = 0;
-    if (hipGetDevice(&cur) != hipSuccess) { ok = false; return; }
+    if (hipGetDevice(&cur) != hipSuccess) {
+      (void)hipGetLastError();
+      ok = false;
+      return;
+    }
     if (cur == dev) return;
     ok = hipSetDevice(dev) == hipSuccess;
     if (ok) before = cur;
+    else (void)hipGetLastError();  // this call's status reports it
   }
   ~Q8KVDevice() {
     if (before >= 0) (void)hipSetDevice(before);

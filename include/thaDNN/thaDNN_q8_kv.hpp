@@ -28,7 +28,7 @@ typedef struct {
   float* vs;
   int n_batches, n_layers, n_kv_heads;
   int head_size;  // 1 .. 256
-  int seq_len;    // positions 0 .. seq_len - 1
+  int seq_len;    // positions 0 .. seq_len - 1; at most 2^30
   int block;      // tokens of a scale: 16, 32, 64 or 128
 } Q8KVCache;
 
@@ -71,7 +71,8 @@ size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batches, int n_to
 // A row at a position outside 0 .. seq_len - 1 sees no key: zeros.  Rows from n_d[b] on are left as they were.
 // q and out are [n_batches][n_tokens][n_heads * head_size] and do not overlap.  work (16-byte aligned) is zeroed once,
 // before its first call (thallama_memset), and then left to these calls, of any shape: each leaves it ready for the next.  It
-// belongs to a call until its kernel has run: calls that may run at once, captured ones among them, have one each.
+// belongs to a call until its kernel has run: calls that may run at once, captured ones among them, have one each.  A
+// call during which pos_d or n_d change leaves it to be zeroed again.
 thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, const Q8KVCache* c, int layer, int n_batches,
                                           int n_tokens, const int* pos_d, const int* n_d, int n_heads,
                                           const float* q, float* out, int q_stride, int out_stride, void* work,

@@ -30,7 +30,7 @@ def test_bytes_and_parts(tl, sizes):
 @pytest.mark.parametrize("sizes", [(0, 1, 1, 64, 64, 16), (1, 0, 1, 64, 64, 16), (1, 1, 0, 64, 64, 16), (1, 1, 1, 0, 64, 16),
                                    (1, 1, 1, 64, 0, 16), (1, 1, 1, 64, 64, 0), (1, 1, 1, 257, 64, 16), (1, 1, 1, 64, 64, 8),
                                    (1, 1, 1, 64, 64, 48), (1, 1, 1, 64, 64, 256), (-1, 1, 1, 64, 64, 16),
-                                   (1, 1, 1, 64, 0x7fffffff, 16), (1 << 30, 1 << 30, 1 << 20, 64, 64, 16),
+                                   (1, 1, 1, 64, 0x7fffffff, 16), (1, 1, 1, 64, 0x40000001, 16), (1 << 30, 1 << 30, 1 << 20, 64, 64, 16),
                                    (1, 1, 1 << 30, 64, 64, 16)])
 def test_no_such_cache(tl, sizes):
     assert tl.lib().thallama_q8_kv_bytes(*sizes) == 0
@@ -82,6 +82,22 @@ def test_refusals(tl, op, change, status):
     ("attention", dict(heads=-4), INVALID), ("attention", dict(BIG, heads=64, qstride=16384, ostride=16384, n=1 << 20), UNSUPPORTED)])
 def test_refusals_of_one(tl, op, change, status):
     assert call(tl, op, **change) == status
+
+
+def test_workspace(tl):
+    """One size serves every call of a cache: it does not shrink with fewer rows or sequences."""
+    size = lambda **c: tl.lib().thaDNN_q8_attention_workspace(  # noqa: E731
+        C.byref(tl.Q8KVCache.make(2, 1, 4, c.get("hs", 64), 100, c.get("block", 32), AT, AT, AT, AT)), c.get("nb", 2), c.get("n", 5), c.get("heads", 8))
+    assert size() > 0 and size(nb=1, n=1, heads=4) == size() == size(n=1000)
+    for bad in (dict(nb=3), dict(nb=0), dict(n=0), dict(heads=6), dict(heads=0), dict(hs=300), dict(block=20)):
+        assert size(**bad) == 0, bad
+    assert tl.lib().thaDNN_q8_attention_workspace(None, 1, 1, 4) == 0
+
+
+@pytest.mark.parametrize("change", [dict(work=None), dict(work=AT + 4), dict(size=64)])
+def test_attention_needs_its_workspace(tl, change):
+    """Few rows over many keys are divided: the call wants the workspace, aligned and whole."""
+    assert call(tl, "attention", **dict(dict(S=4000, n=1), **change)) == INVALID
 
 
 def test_reference_scale_grows():

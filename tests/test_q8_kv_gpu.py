@@ -317,6 +317,46 @@ def test_attention_values_of_very_different_size(gpu, handle, H, nt):
         assert (np.abs(got[b, -1] - want[b, -1]) <= lim).all(), b
 
 
+@pytest.mark.parametrize("first,rest", [(0.0, 1.0), (0.0, 1e4), (1e-37, 1.0), (1e-30, 1e8), (1e30, 1.0)])
+@pytest.mark.parametrize("H,nt", [(2, 1), (2, 40), (130, 70)])  # the last fills the card
+def test_attention_values_that_grow_or_shrink(gpu, handle, first, rest, H, nt):
+    """The first 200 values are zeros, tiny or huge beside the others: the sum of the weights stays whole when the
+    value scales' exponent moves by up to 2^130 from one step to the next."""
+    r = rng(nt)
+    B, hs, S = 2, 64, 400
+    ref = Cache(B, 1, H, hs, S, 32, r)
+    k, v = rows(r, B, S, H, hs) * np.float32(0.3), rows(r, B, S, H, hs)
+    v[:, :200] *= np.float32(first)
+    v[:, 200:] *= np.float32(rest)
+    ref.store(0, [0] * B, [S] * B, k, v)
+    dev = Device(gpu, handle, ref)
+    q = r.standard_normal((B, nt, H, hs)).astype(np.float32)
+    some = [0, nt - 1]
+    got = dev.attend(0, [S - nt] * B, None, q).reshape(q.shape)
+    want, bound = ref.attend(0, [S - nt] * B, [nt] * B, nt, q, 1, some)
+    hold(got[:, some], want[:, some], bound[:, some], f"values {first} then {rest}")
+
+
+def test_attention_scores_of_any_size(gpu, handle):
+    """Scores far below anything a sum starts from (-1e33), and as far above.
+
+    A score is known to 8u of its own size (q8_kv_ref.Cache.attend), u = 2^-24: 1e33 to 5e26, where 1 is a factor of e in
+    its weight.  Every weight from 0 to 1 so lies within the bound, and what is left of it is that a row is some mean of
+    the values: between the least and the largest, up to 400u of the largest for 100 weights held in 24 bits and their sums."""
+    r = rng(1)
+    ref = Cache(2, 1, 1, 64, 100, 16, r)
+    k, v = np.ones((2, 100, 1, 64), np.float32), rows(r, 2, 100, 1, 64)
+    ref.store(0, [0, 0], [100, 100], k, v)
+    dev = Device(gpu, handle, ref)
+    q = np.full((2, 1, 1, 64), 1e32, np.float32)
+    q[0] *= -1
+    got = dev.attend(0, [99, 99], None, q).reshape(2, 64)
+    seen = ref.values("v", 0, np.float64)[:, 0, :100]
+    lim = 400 * 2.0 ** -24 * np.abs(v).max()
+    assert ((got >= seen.min(1) - lim) & (got <= seen.max(1) + lim)).all()
+    assert (np.abs(got).max(1) > 0).all()  # a mean of nothing would be zeros
+
+
 @pytest.mark.parametrize("nt", [1, 20])
 def test_attention_sees_nothing_behind_its_position(gpu, handle, nt):
     """NaN scales and any codes behind the last key leave a row's result bit for bit as it was; a NaN block in sight
@@ -426,6 +466,7 @@ class Hip:
         work()
         self("hipStreamEndCapture", C.c_void_p(stream), C.byref(graph))
         self("hipGraphInstantiate", C.byref(run), graph, None, None, C.c_size_t(0))
+        self("hipGraphDestroy", graph)
         return run
 
 
@@ -488,6 +529,8 @@ def test_captured_decode_step(gpu):
         np.testing.assert_array_equal(got, eager.attend(0, at, None, z).reshape(z.shape), f"replay {t}")
     dev.check("replays")
     eager.check("eager")
+    hip("hipGraphExecDestroy", graph)
+    assert gpu.lib().thablasDestroy(handle) == 0
 
 
 def test_two_streams_at_once(gpu):
@@ -509,6 +552,8 @@ def test_two_streams_at_once(gpu):
     gpu.sync()
     for (_, out, _), want in zip(bufs, alone):
         np.testing.assert_array_equal(out.download(), want.ravel())
+    for h in handles:
+        assert dev.lib.thablasDestroy(h) == 0
 
 
 def test_same_bits_again(gpu, handle):
