@@ -12,10 +12,12 @@
 // sv = f 2^e, 1/2 <= f < 1, the running maximum is taken of x_t + e_t, u_t = 2^(x_t + e_t - M) is at most 1 and
 // n_t = u_t f_t 0x7f7f7f.  The sum of the weights adds u_t 2^(E - e_t), E the largest e so far; value scales under
 // 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not.  M is the maximum of
-// one step's 64 to 256 keys, so that a large weight elsewhere costs the step's own no digits; the steps are summed in fp32.
+// one step's 64 to 256 keys, so that a large weight elsewhere costs the step's own no digits; the steps are summed in
+// fp32.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm), an fp32 softmax over the same
+// codes 3e-7 to 1.8e-6.
 //
-// One i8 product does 16x16x64 in the time in which fp32's does 16x16x8 on eight times the registers; the cache
-// is read as it is, without a conversion.
+// The int8 cores' peak is 5 POP/s beside 157 TFLOP/s for fp32 inputs, so three products are still ten times as fast as
+// one in fp32, and the cache is read as it is, without a conversion.
 //
 // Layout.  S^T = K Q^T and O^T = V^T W^T: a lane holds one query row (column lane & 15) throughout, and with the
 // group g = lane >> 4 the sixteen keys 16g .. 16g + 15 of a tile of 64.  The score product's row m of its j-th
@@ -457,6 +459,12 @@ struct AttnTile {
 // a 64-key tile for each of its waves.  A wave asks for its next keys as soon as the scores are done with these, and for
 // its next values when the sums are.  The waves' results are joined in LDS; where several workgroups share a row tile,
 // each leaves its result in the workspace and the last one to arrive joins them, in the order of the splits whoever it is.
+//
+// Long contexts are bound by memory: eight rows of 32 heads over 8 K/V heads of 128 at 10923 to 32768 keys 65.5 us,
+// 5.5 TB/s of codes (the vector pipe 30% busy), sixteen rows of 32 heads at 683 to 2048 keys 34 us, 5.2 TB/s; codes pass
+// nontemporally (without: 71.5 and 37.9).  Short ones are bound by a chain of latencies: positions, keys, two products
+// and the joins, 12 heads of 64 over 301 keys 5.6 us, 32 of 128 over 2048 keys 9.0 (0.8 until the positions are there,
+// 2.7 to the first codes, 2 for a tile, 0.9 to join the waves, 2.5 the workgroups).
 template <int KS>
 __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_few(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
@@ -571,6 +579,11 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
 // pass through LDS in chunks of NT tiles: the values' codes come in while the scores are computed, the next
 // chunk's keys while the values are.  LDS holds the codes in the order in which the lanes want them, one KiB for
 // each operand of a product, so that a load (16 bytes a lane, memory to LDS) and a read are both linear in the lane.
+//
+// Bound by vector instructions: 340 for 64 keys x 16 rows at heads of 128, beside 48 products that take 768 of their
+// 1400 cycles.  Four 2048-token prompts of 32 heads: 274 us, 501 TFLOP/s of attention (three times that in int8
+// operations), the vector pipe 87% busy at the 1.94 GHz that the card holds under this load.  Two tiles a step leave
+// room for three waves on a SIMD (343 us, four tiles and two waves 352, on one card), heads of 64 fit three with four.
 template <int KS, int NT>
 __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp

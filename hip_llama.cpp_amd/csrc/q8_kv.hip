@@ -109,7 +109,8 @@ struct StoreArgs {
 // A workgroup quantises what the call writes of one (keys or values, sequence, block of tokens) and one or a few
 // heads: thread (head, g, d4) the tokens 16g .. 16g + 15 of the block in dimensions 4*d4 .. + 3, held in registers
 // between the maximum and the codes.  A group of one new token has code of its own: a decode step's store waits for
-// instructions as for anything else.
+// instructions as for anything else (sixteen rows of 32 heads of 128: 5.5 us, with the general code alone 7.3).  Prompts
+// are bound by memory: 8 x 2048 such rows 120 us, 5.6 TB/s of rows in and codes out.
 template <bool VEC>
 __global__ void __launch_bounds__(512) k_q8kv_store(StoreArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
@@ -265,8 +266,8 @@ struct LoadArgs {
   int from;     // 0: keys and values, or keys alone; 1: values alone
 };
 
-// Thread: dimensions d .. d + 3 of one head in the 8 tokens of one group of slots (8 x 2048 rows of 4096, MI355X: 117 us,
-// with 16 tokens 140, with 4 121).
+// Thread: dimensions d .. d + 3 of one head in the 8 tokens of one group of slots.  Bound by memory: 8 x 2048 rows of
+// 4096 117 us, 5.7 TB/s of codes in and rows out (with 16 tokens 140, with 4 121).
 template <bool VEC>
 __global__ void __launch_bounds__(256) k_q8kv_load(LoadArgs a, int both) {
   keep_implicit_args();  // common.hpp
