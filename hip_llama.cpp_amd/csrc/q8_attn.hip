@@ -686,6 +686,15 @@ static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n
   return p;
 }
 
+// A call's rows count in an int, its row tiles in one launch.
+static bool attn_fits(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads) {
+  const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads);
+  const unsigned __int128 pairs = (unsigned __int128)n_batches * c->n_kv_heads;
+  if (rows > 0x7fffffffLL - 64 || !q8kv_grid_ok(pairs * ((rows + 63) / 64), 64 * kWaves)) return false;
+  const AttnPlan p = attn_plan(c, n_batches, n_tokens, n_heads);
+  return q8kv_grid_ok((unsigned __int128)p.units * p.nsplit, 64 * kWaves);
+}
+
 template <int KS>
 static hipError_t attn_launch(const Q8AttnArgs& a, const AttnPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.units * p.nsplit)), block(64 * kWaves);
@@ -710,7 +719,8 @@ static bool attn_sizes_ok(const Q8KVCache* c, int n_heads) {
 
 extern "C" size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads) {
   if (!c || n_batches <= 0 || n_batches > c->n_batches || n_tokens <= 0 || !tl::q8kv_sizes_ok(c->n_batches, c->n_layers, c->n_kv_heads, c->head_size, c->seq_len) ||
-      !tl::q8kv_supported(c->head_size, c->block) || !attn_sizes_ok(c, n_heads))
+      !tl::q8kv_supported(c->head_size, c->block) || !attn_sizes_ok(c, n_heads) ||
+      !tl::attn_fits(c, n_batches, n_tokens, n_heads))
     return 0;
   // a call of fewer rows may divide its keys among more workgroups, but never has more than this many parts
   return tl::kAttnUnits * tl::kCountStep * sizeof(unsigned) + (size_t)2 * tl::kAttnUnits * 16 * tl::attn_part(c->head_size);
@@ -729,8 +739,8 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   if (n_batches == 0 || n_tokens == 0) return THABLAS_STATUS_SUCCESS;
   if (!q || !out) return THABLAS_STATUS_INVALID_VALUE;
   const int mul = n_heads / c->n_kv_heads;
+  if (!tl::attn_fits(c, n_batches, n_tokens, n_heads)) return THABLAS_STATUS_NOT_SUPPORTED;
   const tl::AttnPlan p = tl::attn_plan(c, n_batches, n_tokens, n_heads);
-  if ((long long)n_tokens * mul > 0x7fffffffLL - 64 || p.units * p.nsplit > 0x7fffffffLL / 16) return THABLAS_STATUS_NOT_SUPPORTED;
   const int lrows = (int)min((long long)n_tokens * mul, 16LL);
   const size_t need = p.nsplit > 1 ? tl::kAttnUnits * tl::kCountStep * sizeof(unsigned) + (size_t)p.units * p.nsplit * lrows * tl::attn_part(c->head_size) : 0;
   if (need && (!work || ((uintptr_t)work & 15) || work_bytes < need)) return THABLAS_STATUS_INVALID_VALUE;

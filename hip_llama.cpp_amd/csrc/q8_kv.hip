@@ -336,8 +336,8 @@ extern "C" thablasStatus_t thaDNN_q8_kv_store_batch(thablasHandle_t* handle, con
   a.heads = a.threads < 64 ? 64 / a.threads : 1;
   a.groups = (c->n_kv_heads + a.heads - 1) / a.heads;
   const unsigned __int128 grid = (unsigned __int128)2 * n_batches * a.groups * a.spanned;
-  if (grid > 0x7fffffff) return THABLAS_STATUS_NOT_SUPPORTED;
   const int threads = (a.threads * a.heads + 63) / 64 * 64;
+  if (!tl::q8kv_grid_ok(grid, threads)) return THABLAS_STATUS_NOT_SUPPORTED;
   tl::Q8KVDevice dev(handle->current_gpu_id);
   if (!dev.ok) return THABLAS_STATUS_INVALID_VALUE;
   auto kernel = tl::q8kv_vec4(c->head_size, kv_stride, k, v) ? tl::k_q8kv_store<true> : tl::k_q8kv_store<false>;
@@ -364,7 +364,7 @@ extern "C" thablasStatus_t thaDNN_q8_kv_load_batch(thablasHandle_t* handle, cons
   a.columns = (int)columns;
   const int both = k && v;
   const unsigned __int128 grid = (unsigned __int128)(both ? 2 : 1) * n_batches * a.groups * columns;
-  if (grid > 0x7fffffff) return THABLAS_STATUS_NOT_SUPPORTED;
+  if (!tl::q8kv_grid_ok(grid, 256)) return THABLAS_STATUS_NOT_SUPPORTED;
   tl::Q8KVDevice dev(handle->current_gpu_id);
   if (!dev.ok) return THABLAS_STATUS_INVALID_VALUE;
   auto kernel = tl::q8kv_vec4(c->head_size, kv_stride, k, v) ? tl::k_q8kv_load<true> : tl::k_q8kv_load<false>;

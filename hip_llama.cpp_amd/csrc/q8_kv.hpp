@@ -97,6 +97,9 @@ inline thablasStatus_t q8kv_layer(const thablasHandle_t* handle, const Q8KVCache
   return THABLAS_STATUS_SUCCESS;
 }
 
+// A launch takes fewer than 2^32 threads.
+inline bool q8kv_grid_ok(unsigned __int128 grid, int threads) { return grid * threads <= 0xffffffffu; }
+
 // Rows of `row` floats, `stride` apart, at p: float4 accesses hold if everything is a multiple of 16 bytes.
 inline bool q8kv_vec4(int head_size, int stride, const void* p, const void* q) {
   return head_size % 4 == 0 && stride % 4 == 0 && (((uintptr_t)p | (uintptr_t)q) & 15) == 0;

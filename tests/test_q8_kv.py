@@ -84,6 +84,18 @@ def test_refusals_of_one(tl, op, change, status):
     assert call(tl, op, **change) == status
 
 
+@pytest.mark.parametrize("op,change", [
+    ("store", dict(B=1 << 25, nb=1 << 25, hs=256)), ("load", dict(B=1 << 23, nb=1 << 23, hs=16)),
+    ("attention", dict(B=1 << 24, nb=1 << 24, hs=16)), ("attention", dict(B=1 << 23, nb=1 << 23, n=32, hs=16)), ("attention", dict(B=1 << 20, nb=1 << 20, H=1 << 20, heads=1 << 20, hs=1, n=1 << 30))])
+def test_more_than_a_launch(tl, op, change):
+    """A launch has less than 2^32 threads; rows and heads whose product leaves 64 bits count as more than that."""
+    a = dict(dict(L=1, H=1, S=64, block=16, layer=0, n=1, heads=1), **change)
+    assert call(tl, op, **dict(a, stride=1 << 20, qstride=1 << 20, ostride=1 << 20)) == UNSUPPORTED
+    if op == "attention":
+        cache = tl.Q8KVCache.make(*([a[n] for n in ("B", "L", "H", "hs", "S", "block")] + [AT] * 4))
+        assert tl.lib().thaDNN_q8_attention_workspace(C.byref(cache), a["nb"], a["n"], a["heads"]) == 0
+
+
 def test_workspace(tl):
     """One size serves every call of a cache: it does not shrink with fewer rows or sequences."""
     size = lambda **c: tl.lib().thaDNN_q8_attention_workspace(  # noqa: E731
