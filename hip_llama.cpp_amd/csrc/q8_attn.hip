@@ -430,11 +430,17 @@ TL_DEVICE void lds_wait() {
   __syncthreads();
 }
 
-// A tile of 64 keys as one wave holds it.
-template <int KS>
+// A tile of 64 keys as one wave holds it.  ONCE: no other row tile reads these codes, and they need not stay in L2 (kept
+// there, eight rows over 10923 to 32768 keys take 71.5 us for 65.5; not kept, 256 rows of 32 heads over 16640 keys,
+// sixteen tiles a head, 228 for 167).
+template <int KS, bool ONCE>
 struct AttnTile {
   i4 k[4][KS], v[4 * KS];
   AttnScales<1> c;
+  TL_DEVICE static i4 codes(const int8_t* p) {
+    const i4* q = reinterpret_cast<const i4*>(p);
+    return ONCE ? __builtin_nontemporal_load(q) : *q;
+  }
   TL_DEVICE void load_keys(const Q8AttnArgs& a, const int8_t* k0, const float* ks, const float* vs, int t0, int T) {
     const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
     const int8_t* kp = k0 + (long long)(t0 + 16 * (row >> 2) + (row & 3)) * a.l.lanes;
@@ -444,14 +450,14 @@ struct AttnTile {
 #pragma unroll
       for (int d = 0; d < KS; ++d) {
         const int at = 64 * d + 16 * g;
-        k[j][d] = __builtin_nontemporal_load(reinterpret_cast<const i4*>(kp + 4 * j * a.l.lanes + (at < a.l.lanes ? at : 0)));  // the query's digits are 0 from lanes on
+        k[j][d] = codes(kp + 4 * j * a.l.lanes + (at < a.l.lanes ? at : 0));  // the query's digits are 0 from lanes on
       }
   }
   TL_DEVICE void load_values(const Q8AttnArgs& a, const int8_t* v0, int t0) {
     const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
     const int8_t* vp = v0 + (long long)((t0 >> 4) + g) * (16 * a.l.lanes) + 16 * row;
 #pragma unroll
-    for (int d = 0; d < 4 * KS; ++d) v[d] = __builtin_nontemporal_load(reinterpret_cast<const i4*>(vp + (16 * d < a.l.lanes ? 256 * d : 0)));
+    for (int d = 0; d < 4 * KS; ++d) v[d] = codes(vp + (16 * d < a.l.lanes ? 256 * d : 0));
   }
 };
 
@@ -461,11 +467,10 @@ struct AttnTile {
 // each leaves its result in the workspace and the last one to arrive joins them, in the order of the splits whoever it is.
 //
 // Long contexts are bound by memory: eight rows of 32 heads over 8 K/V heads of 128 at 10923 to 32768 keys 65.5 us,
-// 5.5 TB/s of codes (the vector pipe 30% busy), sixteen rows of 32 heads at 683 to 2048 keys 34 us, 5.2 TB/s; codes pass
-// nontemporally (without: 71.5 and 37.9).  Short ones are bound by a chain of latencies: positions, keys, two products
+// 5.5 TB/s of codes (the vector pipe 30% busy), sixteen rows of 32 heads at 683 to 2048 keys 34 us, 5.2 TB/s.  Short ones are bound by a chain of latencies: positions, keys, two products
 // and the joins, 12 heads of 64 over 301 keys 5.6 us, 32 of 128 over 2048 keys 9.0 (0.8 until the positions are there,
 // 2.7 to the first codes, 2 for a tile, 0.9 to join the waves, 2.5 the workgroups).
-template <int KS>
+template <int KS, bool ONCE>
 __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_few(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -491,7 +496,7 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
   AttnRows<KS> s;
   s.none();
   if (t0 < w.T) {
-    AttnTile<KS> tile;
+    AttnTile<KS, ONCE> tile;
     {
       float x[KS][16];
       const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0, w.rows, w.pos, w.T);
@@ -678,11 +683,12 @@ static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
   // The keys of few tiles are divided until there is a workgroup for each CU, but no further than each wave has a tile (one
-  // row of 32 heads over 2048 keys: 10.4 us; 16 rows: 13.8, with two for each CU 17), or two for each CU where each
-  // wave still has eight (eight 32768-key rows of 8 K/V heads: 66 us, with one 73).
+  // row of 32 heads over 2048 keys: 9.0 us), or two for each CU where each wave still has eight and no other row tile
+  // reads the same keys at its own pace (eight rows of 8 K/V heads over 10923 to 32768 keys: 66 us, with one 73; 32 rows
+  // of 32 heads over 16416, two tiles a head: 46 us, with one 34).
   const long long most = (c->seq_len + 64LL * kWaves - 1) / (64 * kWaves);
   p.nsplit = p.many ? 1 : (int)max(1LL, min(most, min((long long)kMaxSplit, kAttnUnits / p.units)));
-  if (p.nsplit > 1 && most >= 16 * p.nsplit) p.nsplit = min(2 * p.nsplit, kMaxSplit);
+  if (p.nsplit > 1 && p.tiles == 1 && most >= 16 * p.nsplit) p.nsplit = min(2 * p.nsplit, kMaxSplit);
   return p;
 }
 
@@ -702,12 +708,13 @@ static hipError_t attn_launch(const Q8AttnArgs& a, const AttnPlan& p, hipStream_
     hipLaunchKernelGGL((k_q8_attn_many<KS, KS == 1 ? 4 : 2>), grid, block, 0, s, a);
     return hipGetLastError();
   }
+  auto kernel = p.tiles == 1 ? k_q8_attn_few<KS, true> : k_q8_attn_few<KS, false>;
   const size_t lds = (size_t)kWaves * a.lrows * (64 * KS + 4 + 4) * sizeof(float);
   if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)k_q8_attn_few<KS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((k_q8_attn_few<KS>), grid, block, lds, s, a);
+  hipLaunchKernelGGL(kernel, grid, block, lds, s, a);
   return hipGetLastError();
 }
 
