@@ -11,10 +11,11 @@
 // value block's scale, w_t = 2^(x_t - m) sv_t, which is what has to be small beside the row's largest w: with
 // sv = f 2^e, 1/2 <= f < 1, the running maximum is taken of x_t + e_t, u_t = 2^(x_t + e_t - M) is at most 1 and
 // n_t = u_t f_t 0x7f7f7f.  The sum of the weights adds u_t 2^(E - e_t), E the largest e so far; value scales under
-// 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not.  M is the maximum of
-// one step's 64 to 256 keys, so that a large weight elsewhere costs the step's own no digits; the steps are summed in
-// fp32.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm), an fp32 softmax over the same
-// codes 3e-7 to 1.8e-6.
+// 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not; a row is so off by up
+// to 2^-64 of the largest value in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a large weight
+// elsewhere costs the step's own no digits; the steps are summed in fp32, in units of a power that follows M only where
+// it rises past 2^16 of it.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm), an fp32
+// softmax over the same codes 3e-7 to 1.8e-6.
 //
 // The int8 cores' peak is 5 POP/s beside 157 TFLOP/s for fp32 inputs, so three products are still ten times as fast as
 // one in fp32, and the cache is read as it is, without a conversion.
@@ -33,6 +34,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
 constexpr float kNone = -3.4e38f;     // a maximum over nothing
+constexpr float kLag = 16.f;          // log2 of how far a step's maximum may be past the sums' unit
 constexpr int kWaves = 4;             // of a workgroup
 constexpr int kCountStep = 32;        // a cache line for each count of arrivals
 
@@ -51,6 +53,10 @@ struct Q8AttnArgs {
   int vec;           // rows are 16-byte aligned
   float c0;          // log2(e) / sqrt(head_size) / kDigits
 };
+
+// A sum of weights beside values so large that it leaves fp32's range: what is divided by it is under 2^-64 of them either
+// way, and an infinity would not come back from a factor of 0.  A NaN stays.
+TL_DEVICE float sum_kept(float s) { return s > 0x1p120f ? 0x1p120f : s; }
 
 // ---- lanes l, l ^ 16, l ^ 32, l ^ 48 hold one query row
 TL_DEVICE float rows_max(float v) {
@@ -268,10 +274,18 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = fmaxf(m, x[n][j][i]);
   m = rows_max(m);
-  const float M = fmaxf(s.M, m);
-  const float alpha = __builtin_amdgcn_exp2f(s.M - M), beta = __builtin_amdgcn_exp2f(m - M);
-  s.sum = s.sum == 0.f ? 0.f : s.sum * __builtin_amdgcn_exp2f((s.M - M) + (float)grow);  // either alone may be out of range
-  s.M = M;
+  // Rare behind the first step (four prompts of 2048 tokens, 32 heads of 128: 272 us; scaled in each step 276).
+  const float M = m - kLag > s.M ? m : s.M;
+  if (__any(M != s.M || grow)) {
+    const float alpha = __builtin_amdgcn_exp2f(s.M - M);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.o[d][i] *= alpha;
+    s.sum = s.sum == 0.f ? 0.f : s.sum * __builtin_amdgcn_exp2f((s.M - M) + (float)grow);  // either alone may be out of range
+    s.M = M;
+  }
+  const float beta = __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -286,7 +300,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     for (int j = 0; j < 4; ++j) part += (x[n][j][0] + x[n][j][1]) + (x[n][j][2] + x[n][j][3]);
     sum = fmaf(part, c.lift[n], sum);
   }
-  s.sum = fmaf(sum, beta, s.sum);
+  s.sum = sum_kept(fmaf(sum, beta, s.sum));
   i4 p[NT][3];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -301,11 +315,6 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
       p[n][1][j] = p1;
       p[n][2][j] = p2;
     }
-
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s.o[d][i] *= alpha;
 
   ready();
   // values, in the same turns
@@ -390,6 +399,7 @@ TL_DEVICE void parts_join(const f4 (&x)[N], const f4 (&st)[N], int n, f4& o, flo
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], wi, o[e]);
   }
+  sum = sum_kept(sum);
   M = m;
   E = top;
 }
@@ -402,8 +412,8 @@ struct AttnOut {
   TL_DEVICE AttnOut(const Q8AttnArgs& a, const AttnUnit& w, int r, float M, float sum, float E) {
     const int i = (w.r0 + r) / a.mul;
     at = a.out + ((long long)w.b * a.call.n_tokens + i) * a.out_stride + (long long)(w.h * a.mul + w.r0 + r - i * a.mul) * a.l.head_size;
-    inv = M == kNone && sum == 0.f ? 0.f : 1.f / (sum * kDigits);
-    e = (int)E;
+    inv = M == kNone && sum == 0.f ? 0.f : 1.f / (sum * (kDigits * 0x1p-23f));
+    e = (int)E - 23;
   }
   TL_DEVICE void store(const Q8AttnArgs& a, int d, f4 o) const {  // dimensions d .. d + 3
 #pragma unroll
@@ -586,7 +596,7 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
 // each operand of a product, so that a load (16 bytes a lane, memory to LDS) and a read are both linear in the lane.
 //
 // Bound by vector instructions: 340 for 64 keys x 16 rows at heads of 128, beside 48 products that take 768 of their
-// 1400 cycles.  Four 2048-token prompts of 32 heads: 274 us, 501 TFLOP/s of attention (three times that in int8
+// 1400 cycles.  Four 2048-token prompts of 32 heads: 272 us, 505 TFLOP/s of attention (three times that in int8
 // operations), the vector pipe 87% busy at the 1.94 GHz that the card holds under this load.  Two tiles a step leave
 // room for three waves on a SIMD (343 us, four tiles and two waves 352, on one card), heads of 64 fit three with four.
 template <int KS, int NT>

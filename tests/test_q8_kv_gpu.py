@@ -337,6 +337,28 @@ def test_attention_values_that_grow_or_shrink(gpu, handle, first, rest, H, nt):
     hold(got[:, some], want[:, some], bound[:, some], f"values {first} then {rest}")
 
 
+@pytest.mark.parametrize("parts", [(256, 256, 256), (128, 128, 768)])
+@pytest.mark.parametrize("H,nt", [(2, 1), (2, 40), (130, 70)])  # the last fills the card
+def test_attention_scores_that_make_up_for_the_values(gpu, handle, parts, H, nt):
+    """Values of 1e-10, then of 1e30 under scores that leave them nothing (-200), then of 1 under scores of 300: the sum of
+    the weights leaves fp32's range beside the second part's values, and comes back with the third's."""
+    r = rng(nt)
+    B, hs, S = 2, 64, sum(parts)
+    ref = Cache(B, 1, H, hs, S, 64, r)
+    v = rows(r, B, S, H, hs) * np.repeat(np.float32([1e-10, 1e30, 1.0]), parts)[None, :, None, None]
+    k = np.ones((B, S, H, hs), np.float32) * (np.repeat(np.float32([0, -200, 300]), parts) / 8)[None, :, None, None]
+    ref.store(0, [0] * B, [S] * B, k, v)
+    dev = Device(gpu, handle, ref)
+    q = np.ones((B, nt, H, hs), np.float32)
+    some = [0, nt - 1]
+    for seen in (S, parts[0] + parts[1]):  # the third part's keys in sight, and not
+        pos = [seen - nt] * B
+        got = dev.attend(0, pos, None, q).reshape(q.shape)
+        want, bound = ref.attend(0, pos, [nt] * B, nt, q, 1, some)
+        far = 2.0 ** -64 * np.abs(v[:, :seen]).max()
+        hold(got[:, some], want[:, some], bound[:, some] + far, f"{seen} keys")
+
+
 def test_attention_scores_of_any_size(gpu, handle):
     """Scores far below anything a sum starts from (-1e33), and as far above.
 
