@@ -397,6 +397,7 @@ extern "C" int thallama_decoder_create(thallama_decoder** out, const Config* cfg
       why = "batch > 8";
     }
     if (!d->pok && why) d->pwhy = why;
+    if (d->pok) (void)tl::persistent_cooperative();  // found out here: a launch may be captured
   }
   if (!d->mpart_d) {  // split-K scratch of the matrix-core GEMV (batch 1: prefill's short chunks)
     const size_t nblk = (size_t)tl::mfma_target_blocks();

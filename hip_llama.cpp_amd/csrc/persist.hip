@@ -36,6 +36,7 @@
 #include "attention.hpp"
 #include "gemv.hpp"
 #include "gemv_q8.hpp"
+#include "api_lock.hpp"
 #include "persist.hpp"
 
 namespace tl {
@@ -1136,17 +1137,36 @@ bool persistent_prepare(PStep& p, int ncu, const char** why) {
 // (one block per CU), every wait is bounded, and a launch whose waits gave up is reported and
 // re-run on the multi-launch step (tests/test_persist_gpu.py, test_persist_b_gpu.py
 // test_give_up_falls_back: a launch missing a block, eager and from a graph).
-// THALLAMA_PERSIST_COOP=0 selects a plain launch (measurement only).
+// THALLAMA_PERSIST_COOP=0 selects a plain launch (measurement only).  So does a device whose
+// cooperative queue this process cannot have (another process holds it): there a direct launch is
+// refused and a captured one replays without running, so one empty kernel finds out, once per
+// device, before any capture (decoder creation).
+__global__ void k_cooperative_probe() {}
+
+static bool cooperative_queue() {
+  int dev = 0, coop = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&coop, hipDeviceAttributeCooperativeLaunch, dev) != hipSuccess || !coop)
+    return false;
+  ApiLock lock(api_mu());
+  static signed char known[64];  // 1: yes, -1: no
+  if (dev < 64 && known[dev]) return known[dev] > 0;
+  hipStream_t s = nullptr;
+  bool ok = hipStreamCreateWithFlags(&s, hipStreamNonBlocking) == hipSuccess;
+  ok = ok && hipLaunchCooperativeKernel((const void*)k_cooperative_probe, dim3(1), dim3(64), nullptr, 0u, s) == hipSuccess;
+  ok = ok && hipStreamSynchronize(s) == hipSuccess;
+  if (s) (void)hipStreamDestroy(s);
+  if (!ok) (void)hipGetLastError();  // (not sticky for the caller's next launch check)
+  if (dev < 64) known[dev] = ok ? 1 : -1;
+  return ok;
+}
+
 static bool use_cooperative() {
-  static const bool on = [] {
+  static const bool off = [] {
     const char* e = getenv("THALLAMA_PERSIST_COOP");
-    int dev = 0, coop = 0;
-    if (hipGetDevice(&dev) != hipSuccess ||
-        hipDeviceGetAttribute(&coop, hipDeviceAttributeCooperativeLaunch, dev) != hipSuccess)
-      coop = 0;
-    return coop != 0 && !(e && e[0] == '0');
+    return e && e[0] == '0';
   }();
-  return on;
+  return !off && cooperative_queue();
 }
 
 bool persistent_cooperative() { return use_cooperative(); }
