@@ -595,9 +595,9 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
 // chunk's keys while the values are.  LDS holds the codes in the order in which the lanes want them, one KiB for
 // each operand of a product, so that a load (16 bytes a lane, memory to LDS) and a read are both linear in the lane.
 //
-// Bound by vector instructions: 340 for 64 keys x 16 rows at heads of 128, beside 48 products that take 768 of their
-// 1400 cycles.  Four 2048-token prompts of 32 heads: 272 us, 505 TFLOP/s of attention (three times that in int8
-// operations), the vector pipe 87% busy at the 1.94 GHz that the card holds under this load.  Two tiles a step leave
+// Bound by vector instructions and by power: 64 keys x 16 rows at heads of 128 take a SIMD 2070 cycles, of which 370 vector
+// instructions fill 1660 and 48 products, beside them, 768.  Four 2048-token prompts of 32 heads: 272 us, 505 TFLOP/s of attention (three times that in int8
+// operations), the vector pipe 84% busy at the 1.94 GHz that the card holds under this load.  Two tiles a step leave
 // room for three waves on a SIMD (343 us, four tiles and two waves 352, on one card), heads of 64 fit three with four.
 template <int KS, int NT>
 __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs a) {
