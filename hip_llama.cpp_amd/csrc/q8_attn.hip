@@ -477,9 +477,10 @@ struct AttnTile {
 // each leaves its result in the workspace and the last one to arrive joins them, in the order of the splits whoever it is.
 //
 // Long contexts are bound by memory: eight rows of 32 heads over 8 K/V heads of 128 at 10923 to 32768 keys 65.5 us,
-// 5.5 TB/s of codes (the vector pipe 30% busy), sixteen rows of 32 heads at 683 to 2048 keys 34 us, 5.2 TB/s.  Short ones are bound by a chain of latencies: positions, keys, two products
-// and the joins, 12 heads of 64 over 301 keys 5.6 us, 32 of 128 over 2048 keys 9.0 (0.8 until the positions are there,
-// 2.7 to the first codes, 2 for a tile, 0.9 to join the waves, 2.5 the workgroups).
+// 5.5 TB/s of codes (the vector pipe 30% busy), sixteen rows of 32 heads at 683 to 2048 keys 34 us, 5.2 TB/s.  Short ones
+// are bound by a chain of latencies: positions, keys, two products and the joins, 12 heads of 64 over 301 keys 5.8 us, 32
+// of 128 over 2048 keys 9.1 (0.8 until the positions are there, 2.7 to the first codes, 2 for a tile, 0.9 to join the
+// waves, 2.5 the workgroups).
 template <int KS, bool ONCE>
 __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_few(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp: rocprofv3 --pmc needs the hidden kernargs
@@ -595,10 +596,11 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
 // chunk's keys while the values are.  LDS holds the codes in the order in which the lanes want them, one KiB for
 // each operand of a product, so that a load (16 bytes a lane, memory to LDS) and a read are both linear in the lane.
 //
-// Bound by vector instructions and by power: 64 keys x 16 rows at heads of 128 take a SIMD 2070 cycles, of which 370 vector
-// instructions fill 1660 and 48 products, beside them, 768.  Four 2048-token prompts of 32 heads: 272 us, 505 TFLOP/s of attention (three times that in int8
-// operations), the vector pipe 84% busy at the 1.94 GHz that the card holds under this load.  Two tiles a step leave
-// room for three waves on a SIMD (343 us, four tiles and two waves 352, on one card), heads of 64 fit three with four.
+// Bound by vector instructions and by power: 64 keys x 16 rows at heads of 128 take a SIMD 2070 cycles, of which 370
+// vector instructions fill 1660 and 48 products, beside them, 768.  Four 2048-token prompts of 32 heads: 272 us, 505
+// TFLOP/s of attention (three times that in int8 operations), the vector pipe 84% busy at the 1.94 GHz that the card
+// holds under this load.  Two tiles a step leave room for three waves on a SIMD (343 us, four tiles and two waves 352, on
+// one card), heads of 64 fit three with four.
 template <int KS, int NT>
 __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp
@@ -688,12 +690,13 @@ static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n
   const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads), pairs = (long long)n_batches * c->n_kv_heads;
   // Tiles of 64 rows that fill the card go to k_q8_attn_many: from 256 of them on (256, of 32 heads x 512 rows: 16.5 us,
   // k_q8_attn_few 19.1; 224: 15.1 and 16.1; 352: 22.4 and 28.6), at heads of up to 64, where the few rows' kernel fits
-  // four waves on a SIMD, from 512 (264, of 12 heads x 1400 rows: 24.0 us and 17.4; 564: 47.1 and 49.5).
+  // four waves on a SIMD, from 512 (264, of 12 heads x 1400 rows: 24.0 us and 17.3; 528, of two
+  // sequences: 26.5 and 27.5).
   p.many = rows >= 64 && pairs * ((rows + 63) / 64) >= (c->head_size <= 64 ? 2 : 1) * kAttnUnits;
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
   // The keys of few tiles are divided until there is a workgroup for each CU, but no further than each wave has a tile (one
-  // row of 32 heads over 2048 keys: 9.0 us), or two for each CU where each wave still has eight and no other row tile
+  // row of 32 heads over 2048 keys: 9.1 us), or two for each CU where each wave still has eight and no other row tile
   // reads the same keys at its own pace (eight rows of 8 K/V heads over 10923 to 32768 keys: 66 us, with one 73; 32 rows
   // of 32 heads over 16416, two tiles a head: 46 us, with one 34).
   const long long most = (c->seq_len + 64LL * kWaves - 1) / (64 * kWaves);
