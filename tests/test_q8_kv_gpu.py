@@ -610,3 +610,21 @@ def test_offsets_past_32_bits(gpu, handle):
     for w in "kv":
         np.testing.assert_array_equal(back[w][B - 1], small.values(w, 0)[B - 1, :, :nt].transpose(1, 0, 2).reshape(nt, -1))
         assert (back[w][:B - 1] == -77).all()
+
+
+def test_fewer_sequences_than_the_cache_holds(gpu, handle):
+    """A call works on the first sequences alone, in the order of the cache's."""
+    r = rng(3)
+    ref, dev = filled(gpu, handle, r, 4, 2, 2, 32, 150, 32, [60, 70, 80, 90], 1)
+    x, y = rows(r, 2, 9, 2, 32), rows(r, 2, 9, 2, 32)
+    ref.store(1, [60, 70], [9, 9], x, y)
+    dev.store(1, [60, 70], None, x, y)
+    dev.check("two of four")
+    q = r.standard_normal((2, 9, 4, 32)).astype(np.float32)
+    want, bound = ref.attend(1, [60, 70], [9, 9], 9, q, 2)
+    hold(dev.attend(1, [60, 70], None, q).reshape(q.shape), want, bound, "two of four")
+    back = dev.load(1, [0, 5], None, 40)
+    for w in "kv":
+        all_of = ref.values(w, 1)
+        for b, first in enumerate([0, 5]):
+            np.testing.assert_array_equal(back[w][b].reshape(40, 2, 32), all_of[b, :, first:first + 40].transpose(1, 0, 2))
