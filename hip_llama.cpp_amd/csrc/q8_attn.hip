@@ -10,7 +10,7 @@
 // row's largest |q|: off by 2^-24 of that, as an fp32 number is.  For the values it is the softmax weight times the
 // value block's scale, w_t = 2^(x_t - m) sv_t, which is what has to be small beside the row's largest w: with
 // sv = f 2^e, 1/2 <= f < 1, the running maximum is taken of x_t + e_t, u_t = 2^(x_t + e_t - M) is at most 1 and
-// n_t = u_t f_t 0x7f7f7f.  The sum of the weights adds u_t 2^(E - e_t), E the largest e so far; value scales under
+// n_t = u_t f_t 0x7f7f7f.  The sum of the weights adds u_t 2^(E - e_t), E the row's largest e so far; value scales under
 // 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not; a row is so off by up
 // to 2^-64 of the largest value in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a large weight
 // elsewhere costs the step's own no digits; the steps are summed in fp32, in units of a power that follows M only where
@@ -99,7 +99,7 @@ struct AttnRows {
   int seen;      // keys that the row sees
   float M, sum;  // running maximum, sum of weights
   f4 o[4 * KS];  // sums over the values: dimensions 16 d + 4 (lane >> 4) .. + 3
-  int E;         // largest value exponent
+  int E;         // largest value exponent that the row has seen
 
   TL_DEVICE void none() {  // before the first key
     M = kNone;
@@ -195,10 +195,12 @@ template <int KS, int NT, class Key, class Val, class Ready>
 TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
   constexpr int DT = 4 * KS;
   const int g = (threadIdx.x & 63) >> 4;
+  const int left = s.seen - t0 - 16 * g;  // keys of this lane's first tile and behind it that the row sees
   int top = s.E, grow = 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     c.e[n] = c.f[n] > 0.f ? __builtin_amdgcn_frexp_expf(c.f[n]) : -126;
+    if (edge && 64 * n >= left) c.e[n] = -126;  // a row's exponent goes by what it sees
     top = max(top, c.e[n]);
   }
   if (__any(top > s.E)) {  // rare behind the first step
@@ -253,7 +255,6 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     }
   }
 
-  const int left = s.seen - t0 - 16 * g;  // keys of this lane's first tile and behind it that the row sees
   if (edge) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)

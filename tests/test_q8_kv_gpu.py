@@ -337,6 +337,28 @@ def test_attention_values_that_grow_or_shrink(gpu, handle, first, rest, H, nt):
     hold(got[:, some], want[:, some], bound[:, some], f"values {first} then {rest}")
 
 
+@pytest.mark.parametrize("first", [0.0, 1e-37, 1e-30])
+@pytest.mark.parametrize("H,nt", [(2, 40), (130, 70)])  # the last fills the card
+def test_attention_rows_that_end_before_larger_values(gpu, handle, first, H, nt):
+    """Rows that see only zeros, or tiny values, beside rows of the same call that see larger ones in the keys behind: each
+    row's sum of the weights goes by the values that it sees itself.  Every row's last key falls into the turn from one to
+    the other, at a tile's first key and inside a tile."""
+    r = rng(nt)
+    B, hs, S, block = 2, 64, 400, 32
+    ref = Cache(B, 1, H, hs, S, block, r)
+    k, v = rows(r, B, S, H, hs) * np.float32(0.3), rows(r, B, S, H, hs)
+    ends = [384 - nt // 2, 352 - nt // 2]
+    for b in range(B):
+        v[b, 100:ends[b] + nt // 2] *= np.float32(first)
+    ref.store(0, [0] * B, [S] * B, k, v)
+    dev = Device(gpu, handle, ref)
+    q = r.standard_normal((B, nt, H, hs)).astype(np.float32)
+    got = dev.attend(0, ends, None, q).reshape(q.shape)
+    some = range(nt) if H < 100 else range(0, nt, 9)
+    want, bound = ref.attend(0, ends, [nt] * B, nt, q, 1, some)
+    hold(got[:, some], want[:, some], bound[:, some], f"values {first}")
+
+
 @pytest.mark.parametrize("parts", [(256, 256, 256), (128, 128, 768)])
 @pytest.mark.parametrize("H,nt", [(2, 1), (2, 40), (130, 70)])  # the last fills the card
 def test_attention_scores_that_make_up_for_the_values(gpu, handle, parts, H, nt):
