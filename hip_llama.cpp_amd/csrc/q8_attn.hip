@@ -12,10 +12,10 @@
 // sv = f 2^e, 1/2 <= f < 1, the running maximum is taken of x_t + e_t, u_t = 2^(x_t + e_t - M) is at most 1 and
 // n_t = u_t f_t 0x7f7f7f.  The sum of the weights adds u_t 2^(E - e_t), E the row's largest e so far; value scales under
 // 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not; a row is so off by up
-// to 2^-64 of 127 of the largest value scale in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a large weight
-// elsewhere costs the step's own no digits; the steps are summed in fp32, in units of a power that follows M only where
-// it rises past 2^16 of it.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm), an fp32
-// softmax over the same codes 3e-7 to 1.8e-6.
+// to 2^-64 of 127 of the largest value scale in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a
+// large weight elsewhere costs the step's own no digits; the steps are summed in fp32, in units of a power that follows
+// M only where it rises past 2^16 of it.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm),
+// an fp32 softmax over the same codes 3e-7 to 1.8e-6.
 //
 // The int8 cores' peak is 5 POP/s beside 157 TFLOP/s for fp32 inputs, so three products are still ten times as fast as
 // one in fp32, and the cache is read as it is, without a conversion.
