@@ -35,6 +35,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
 constexpr float kNone = -3.4e38f;     // a maximum over nothing
 constexpr float kLag = 16.f;          // log2 of how far a step's maximum may be past the sums' unit
+constexpr int kUnit = 28;             // power of two in c0, so that its product with a key scale is a normal float
 constexpr int kWaves = 4;             // of a workgroup
 constexpr int kCountStep = 32;        // a cache line for each count of arrivals
 
@@ -51,7 +52,7 @@ struct Q8AttnArgs {
   int nsplit;        // workgroups that share a row tile's keys
   int lrows;         // rows of a tile that any sequence can have
   int vec;           // rows are 16-byte aligned
-  float c0;          // log2(e) / sqrt(head_size) / kDigits
+  float c0;          // log2(e) / sqrt(head_size) / kDigits 2^kUnit: 2.9 .. 46
 };
 
 // A sum of weights beside values so large that it leaves fp32's range: what is divided by it is under 2^-64 of them either
@@ -94,7 +95,7 @@ TL_DEVICE i4 mfma(i4 a, i4 b, i4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_
 template <int KS>
 struct AttnRows {
   i4 q[3][KS];   // query digits, lowest first
-  int qe;        // their power of two
+  int qe;        // their power of two, less kUnit
   float qn;      // 1, or NaN for a query that is not finite
   int seen;      // keys that the row sees
   float M, sum;  // running maximum, sum of weights
@@ -157,14 +158,15 @@ TL_DEVICE void attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
     for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
   top = rows_umax(top);
   s.qn = top < 0x7f800000u ? 1.f : __builtin_nanf("");
-  s.qe = top < 0x7f800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
+  const int qe = top < 0x7f800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
+  s.qe = qe - kUnit;
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       unsigned n[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) n[c] = (unsigned)(int)rintf(__builtin_ldexpf(x[k][4 * e + c], -s.qe) * kDigits) + 0x8080u;
+      for (int c = 0; c < 4; ++c) n[c] = (unsigned)(int)rintf(__builtin_ldexpf(x[k][4 * e + c], -qe) * kDigits) + 0x8080u;
       int p0, p1, p2;
       digits4(n, p0, p1, p2);
       s.q[0][k][e] = p0;
@@ -778,7 +780,7 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   a.nsplit = p.nsplit;
   a.lrows = lrows;
   a.vec = tl::q8kv_vec4(c->head_size, q_stride, q, out) && out_stride % 4 == 0;
-  a.c0 = (float)(1.4426950408889634 / __builtin_sqrt((double)c->head_size) / tl::kDigits);
+  a.c0 = (float)__builtin_ldexp(1.4426950408889634 / __builtin_sqrt((double)c->head_size) / tl::kDigits, tl::kUnit);
   tl::Q8KVDevice dev(handle->current_gpu_id);
   if (!dev.ok) return THABLAS_STATUS_INVALID_VALUE;
   const int ks = (a.l.lanes + 63) / 64;
