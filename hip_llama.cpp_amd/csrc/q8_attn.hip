@@ -14,7 +14,9 @@
 // 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not; a row is so off by up
 // to 2^-64 of 127 of the largest value scale in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a
 // large weight elsewhere costs the step's own no digits; the steps are summed in fp32, in units of a power that follows
-// M only where it rises past 2^16 of it.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm),
+// M only where it rises past 2^16 of it.  A large weight on a key of small values still costs its neighbours theirs (the
+// first token of a model, with nearly all of a row's weight and nothing in its values: without more, the row would be 4e-5 to 1e-1
+// off): where a step leaves a row's sums small its weights get three more digits behind these.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm),
 // an fp32 softmax over the same codes 3e-7 to 1.8e-6.
 //
 // The int8 cores' peak is 5 POP/s beside 157 TFLOP/s for fp32 inputs, so three products are still ten times as fast as
@@ -33,9 +35,11 @@ namespace tl {
 typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr float kDigits = 8355711.f;  // 0x7f7f7f, the largest n whose balanced digits fit three signed bytes
+constexpr float kRound = 8421504.f;   // 2^23 + 0x8080: a sum with it is rounded to a whole number
 constexpr float kNone = -3.4e38f;     // a maximum over nothing
 constexpr float kLag = 16.f;          // log2 of how far a step's maximum may be past the sums' unit
 constexpr int kUnit = 28;             // power of two in c0, so that its product with a key scale is a normal float
+constexpr float kFew = 0x1p26f;       // sums of a row under this many of a step's units: its weights' further digits count
 constexpr int kWaves = 4;             // of a workgroup
 constexpr int kCountStep = 32;        // a cache line for each count of arrivals
 
@@ -180,8 +184,8 @@ template <int NT>
 struct AttnScales {
   float sk[NT], f[NT], lift[NT];
   int e[NT];
-  TL_DEVICE void load(const Q8AttnArgs& a, const float* ks, const float* vs, int t0, int T) {
-    const unsigned g16 = threadIdx.x & 48u, last = (unsigned)(T - 1);
+  TL_DEVICE void load(const Q8AttnArgs& a, const float* ks, const float* vs, int lane, int t0, int T) {
+    const unsigned g16 = lane & 48, last = (unsigned)(T - 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const unsigned j = min(t0 + 64u * n + g16, last) >> a.l.block_log2;
@@ -189,40 +193,51 @@ struct AttnScales {
       f[n] = vs[j];
     }
   }
+  // Exponents of the value scales, as far as the row sees their keys (`left` of them, counted from the lane's first tile
+  // on): a row's exponent goes by what it sees.
+  TL_DEVICE void exponents(bool edge, int left) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      e[n] = f[n] > 0.f ? __builtin_amdgcn_frexp_expf(f[n]) : -126;
+      if (edge && 64 * n >= left) e[n] = -126;
+    }
+  }
+  // Their factors, once the row's largest exponent E is known.
+  TL_DEVICE void factors(int E) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      e[n] = max(e[n], E - 40);
+      lift[n] = f[n] == f[n] ? __builtin_ldexpf(1.f, E - e[n]) : f[n];  // a NaN scale makes the sum NaN
+      f[n] = __builtin_ldexpf(f[n], -e[n]) * kDigits;
+    }
+  }
 };
 
-// One step of NT tiles of 64 keys from t0 on.  Key: (tile, 16-key step, 64-dimension step), Val: (tile, 16-dimension
-// step) -> sixteen codes.  ready() runs between the two products.
-template <int KS, int NT, class Key, class Val, class Ready>
-TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
-  constexpr int DT = 4 * KS;
-  const int g = (threadIdx.x & 63) >> 4;
-  const int left = s.seen - t0 - 16 * g;  // keys of this lane's first tile and behind it that the row sees
-  int top = s.E, grow = 0;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    c.e[n] = c.f[n] > 0.f ? __builtin_amdgcn_frexp_expf(c.f[n]) : -126;
-    if (edge && 64 * n >= left) c.e[n] = -126;  // a row's exponent goes by what it sees
-    top = max(top, c.e[n]);
-  }
-  if (__any(top > s.E)) {  // rare behind the first step
-    v2u r = __builtin_amdgcn_permlane32_swap((unsigned)top, (unsigned)top, false, false);
-    top = max((int)r.x, (int)r.y);
-    r = __builtin_amdgcn_permlane16_swap((unsigned)top, (unsigned)top, false, false);
-    top = max((int)r.x, (int)r.y);
-    grow = top - s.E;
-    s.E = top;
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    c.e[n] = max(c.e[n], top - 40);
-    c.lift[n] = c.f[n] == c.f[n] ? __builtin_ldexpf(1.f, top - c.e[n]) : c.f[n];  // a NaN scale makes the sum NaN
-    c.f[n] = __builtin_ldexpf(c.f[n], -c.e[n]) * kDigits;
-  }
+struct AttnUnit {  // what a workgroup works on
+  int b, h, r0, rows, nr, T;
+  long long pos;
+};
+// Row tile `tile` of R rows of pair (b, h); false if the sequence has no such rows.
+TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, AttnUnit& w) {
+  w.h = pair % a.l.heads;
+  w.b = pair / a.l.heads;
+  int count;
+  q8kv_start(a.call, w.b, w.pos, count);
+  w.rows = count * a.mul;
+  w.r0 = tile * R;
+  if (w.r0 >= w.rows) return false;
+  w.nr = min(R, w.rows - w.r0);
+  const long long first = w.pos + w.r0 / a.mul, last = w.pos + (w.r0 + w.nr - 1) / a.mul;
+  w.T = first >= a.l.seq_len ? 0 : (int)max(0LL, min(last + 1, (long long)a.l.seq_len));
+  return true;
+}
 
-  // Scores.  Each turn asks for the next one's operands, starts this one's products and finishes the last one's, so
-  // that neither LDS nor the matrix pipe is waited for.
-  f4 x[NT][4];
+// Scores x_t + e_t of NT tiles of 64 keys, -inf for those that the row does not see, whose factors become 0.
+// key: (tile, 16-key step, 64-dimension step) -> sixteen codes.
+template <int KS, int NT, class Key>
+TL_DEVICE void attn_scores(f4 (&x)[NT][4], AttnScales<NT>& c, const AttnRows<KS>& s, const Q8AttnArgs& a, bool edge, int left, Key key) {
+  // Each turn asks for the next one's operands, starts this one's products and finishes the last one's, so that neither
+  // LDS nor the matrix pipe is waited for.
   {
     i4 k[2][KS], acc[2][3];
     float c1 = 0.f, ce = 0.f;
@@ -256,27 +271,106 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+  if (!edge) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (64 * n + 4 * j + i >= left) x[n][j][i] = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    if (64 * n >= left) c.f[n] = c.lift[n] = 0.f;  // a block behind the row may hold NaN
+}
 
-  if (edge) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (64 * n + 4 * j + i >= left) x[n][j][i] = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      if (64 * n >= left) c.f[n] = c.lift[n] = 0.f;  // a block behind the row may hold NaN
-  }
-  float m = kNone;  // of this step alone: it sets the size that the step's weights are rounded to
+// The largest score of the row.
+template <int NT>
+TL_DEVICE float attn_most(const f4 (&x)[NT][4]) {
+  float m = kNone;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = fmaxf(m, x[n][j][i]);
-  m = rows_max(m);
+  return rows_max(m);
+}
+
+// o += beta sum n_t v_t of NT tiles, n_t in the digits p.  val: (tile, 16-dimension step) -> sixteen codes; turns as above.
+template <int KS, int NT, class Val>
+TL_DEVICE void attn_values(f4 (&o)[4 * KS], const i4 (&p)[NT][3], float beta, Val val) {
+  constexpr int DT = 4 * KS;
+  i4 v[2][NT], acc[2][3];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) v[0][n] = val(n, 0);
+#pragma unroll
+  for (int u = 0; u <= DT; ++u) {
+    if (u + 1 < DT) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) v[(u + 1) & 1][n] = val(n, u + 1);
+    }
+    if (u < DT) {
+#pragma unroll
+      for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(v[u & 1][0], p[0][z], i4{0, 0, 0, 0});
+#pragma unroll
+      for (int n = 1; n < NT; ++n)
+#pragma unroll
+        for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(v[u & 1][n], p[n][z], acc[u & 1][z]);
+    }
+    if (u > 0) {
+      const i4(&r)[3] = acc[(u - 1) & 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        o[u - 1][i] = fmaf(fmaf((float)r[2][i], 65536.f, (float)((r[1][i] << 8) + r[0][i])), beta, o[u - 1][i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The codes of a (sequence, K/V head), and the keys that a workgroup's rows see.
+struct AttnHead {
+  const int8_t *k, *v;
+  const float *ks, *vs;
+  int T;
+  TL_DEVICE AttnHead(const Q8AttnArgs& a, const AttnUnit& w)
+      : k(a.l.k + w.b * a.l.seq_codes + w.h * a.l.head_codes), v(a.l.v + w.b * a.l.seq_codes + w.h * a.l.head_codes),
+        ks(a.l.ks + w.b * a.l.seq_scales + w.h * a.l.head_scales), vs(a.l.vs + w.b * a.l.seq_scales + w.h * a.l.head_scales), T(w.T) {}
+  // This lane's operands of the tile at t0: key step j and dimension step d, values' dimension step d.  Behind the lanes
+  // the first ones again: the query's digits are 0 there, and such values are no row's.
+  TL_DEVICE const int8_t* key(const Q8AttnArgs& a, int lane, int t0, int j, int d) const {
+    const int row = lane & 15, at = 64 * d + 16 * (lane >> 4);
+    return k + (long long)(t0 + 16 * (row >> 2) + (row & 3)) * a.l.lanes + 4 * j * a.l.lanes + (at < a.l.lanes ? at : 0);
+  }
+  TL_DEVICE const int8_t* value(const Q8AttnArgs& a, int lane, int t0, int d) const {
+    const int row = lane & 15, g = lane >> 4;
+    return v + (long long)((t0 >> 4) + g) * (16 * a.l.lanes) + 16 * row + (16 * d < a.l.lanes ? 256 * d : 0);
+  }
+};
+
+// One step of NT tiles of 64 keys from t0 on; key and val as above.  ready() runs between the two products.  The rows of
+// the wave whose weights need further digits, as bits.
+template <int KS, int NT, class Key, class Val, class Ready>
+TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
+  constexpr int DT = 4 * KS;
+  const int g = (threadIdx.x & 63) >> 4;
+  const int left = s.seen - t0 - 16 * g;  // keys of this lane's first tile and behind it that the row sees
+  int top = s.E, grow = 0;
+  c.exponents(edge, left);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) top = max(top, c.e[n]);
+  if (__any(top > s.E)) {  // rare behind the first step
+    v2u r = __builtin_amdgcn_permlane32_swap((unsigned)top, (unsigned)top, false, false);
+    top = max((int)r.x, (int)r.y);
+    r = __builtin_amdgcn_permlane16_swap((unsigned)top, (unsigned)top, false, false);
+    top = max((int)r.x, (int)r.y);
+    grow = top - s.E;
+    s.E = top;
+  }
+  c.factors(s.E);
+  f4 x[NT][4];
+  attn_scores<KS, NT>(x, c, s, a, edge, left, key);
+  const float m = attn_most<NT>(x);  // of this step alone: it sets the size that the step's weights are rounded to
   // Rare behind the first step (four prompts of 2048 tokens, 32 heads of 128: 272 us; scaled in each step 276).
   const float M = m - kLag > s.M ? m : s.M;
   if (__any(M != s.M || grow)) {
@@ -311,7 +405,7 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     for (int j = 0; j < 4; ++j) {
       unsigned w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmaf(x[n][j][i], c.f[n], 8421504.f));  // 2^23 + 0x8080: low bytes n + 0x8080, rounded to nearest
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmaf(x[n][j][i], c.f[n], kRound));  // low bytes n + 0x8080, rounded to nearest
       int p0, p1, p2;
       digits4(w, p0, p1, p2);
       p[n][0][j] = p0;
@@ -320,34 +414,18 @@ TL_DEVICE void attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c
     }
 
   ready();
-  // values, in the same turns
-  {
-    i4 v[2][NT], acc[2][3];
+  attn_values<KS, NT>(s.o, p, beta, val);
+
+  // Too few digits?  Half a unit for each n_t of 64 to 256 keys, of codes up to 127 and about 30 in the mean, is some 50 to
+  // 130 units beside the row's sums, which are about 2^28 where one key's ordinary codes are all that counts.  Looked at in
+  // the first 32 dimensions, or 16 of fewer; lanes whose four of these go past the head's end have no say.
+  const float second = KS > 1 || a.l.head_size >= 32 ? 1.f : 0.f;
+  float most = 0.f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) v[0][n] = val(n, 0);
-#pragma unroll
-    for (int u = 0; u <= DT; ++u) {
-      if (u + 1 < DT) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) v[(u + 1) & 1][n] = val(n, u + 1);
-      }
-      if (u < DT) {
-#pragma unroll
-        for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(v[u & 1][0], p[0][z], i4{0, 0, 0, 0});
-#pragma unroll
-        for (int n = 1; n < NT; ++n)
-#pragma unroll
-          for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(v[u & 1][n], p[n][z], acc[u & 1][z]);
-      }
-      if (u > 0) {
-        const i4(&r)[3] = acc[(u - 1) & 1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s.o[u - 1][i] = fmaf(fmaf((float)r[2][i], 65536.f, (float)((r[1][i] << 8) + r[0][i])), beta, s.o[u - 1][i]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
+  for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(s.o[0][i]), fabsf(s.o[1][i]) * second));
+  unsigned long long few = __ballot((most < kFew * beta || (KS == 1 && 4 * g + 4 > a.l.head_size)) && m > kNone);
+  few &= few >> 32;
+  return (unsigned)(few & (few >> 16)) & 0xffffu;  // all four lanes of a row
 }
 
 // The least number of keys that one of the wave's rows sees.
@@ -359,23 +437,70 @@ TL_DEVICE int attn_least(int seen) {
   return __builtin_amdgcn_readfirstlane(seen);
 }
 
-struct AttnUnit {  // what a workgroup works on
-  int b, h, r0, rows, nr, T;
-  long long pos;
+// In which of a wave's steps, `step` keys apart and together T, the lane's row needs further digits for its weights: a bit
+// for each, or for several where they are more than 32.  A row's own, so that no row depends on its neighbours in the tile.
+struct AttnMarks {
+  unsigned bits = 0;
+  int shift;
+  TL_DEVICE AttnMarks(int T, int step) : shift(max(0, __builtin_clz((unsigned)step) - __builtin_clz((unsigned)T | 1u) - 4)) {}
+  TL_DEVICE void mark(int i, unsigned rows) { bits |= ((rows >> (threadIdx.x & 15)) & 1u) << (i >> shift); }
 };
-// Row tile `tile` of R rows of pair (b, h); false if the sequence has no such rows.
-TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, AttnUnit& w) {
-  w.h = pair % a.l.heads;
-  w.b = pair / a.l.heads;
-  int count;
-  q8kv_start(a.call, w.b, w.pos, count);
-  w.rows = count * a.mul;
-  w.r0 = tile * R;
-  if (w.r0 >= w.rows) return false;
-  w.nr = min(R, w.rows - w.r0);
-  const long long first = w.pos + w.r0 / a.mul, last = w.pos + (w.r0 + w.nr - 1) / a.mul;
-  w.T = first >= a.l.seq_len ? 0 : (int)max(0LL, min(last + 1, (long long)a.l.seq_len));
-  return true;
+
+// What a step's weights have beyond their 24 bits: u_t f_t 0x7f7f7f - n_t, at most 1/2, in three more digits of 2^-24 each.
+// A row needs it where one key has far more weight than others and next to nothing in its values (a model's first token),
+// in the steps that hold such a key.  Its operands are read again when all keys are through, and taken tile by tile: in the
+// loop itself the registers would be short.
+template <int KS, int NT>
+TL_DEVICE void attn_further(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnHead& h, int t0, bool edge, bool mine) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // addresses are made here, not ahead and kept in registers
+  const int left = s.seen - t0 - 16 * (lane >> 4), tiles = min(NT, (h.T - t0 + 63) / 64);
+  f4 x[1][4];
+  AttnScales<1> c;
+  auto scores = [&](int n) {
+    c.load(a, h.ks, h.vs, lane, t0 + 64 * n, h.T);
+    c.exponents(edge, left - 64 * n);
+    c.factors(s.E);
+    attn_scores<KS, 1>(x, c, s, a, edge, left - 64 * n, [&](int, int j, int d) { return *reinterpret_cast<const i4*>(h.key(a, lane, t0 + 64 * n, j, d)); });
+  };
+  float m = kNone;  // the step's
+#pragma unroll 1
+  for (int n = 0; n < tiles; ++n) {
+    scores(n);
+    m = fmaxf(m, attn_most<1>(x));
+  }
+#pragma unroll 1
+  for (int n = 0; n < tiles; ++n) {
+    if (NT > 1) scores(n);
+    i4 p[1][3];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unsigned w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float u = __builtin_amdgcn_exp2f(x[0][j][i] - m);
+        const float whole = fmaf(u, c.f[0], kRound) - kRound;
+        w[i] = (unsigned)(int)rintf(fmaf(u, c.f[0], -whole) * (2.f * kDigits)) + 0x8080u;
+      }
+      int p0, p1, p2;
+      digits4(w, p0, p1, p2);
+      p[0][0][j] = p0;
+      p[0][1][j] = p1;
+      p[0][2][j] = p2;
+    }
+    attn_values<KS, 1>(s.o, p, mine ? __builtin_amdgcn_exp2f(m - s.M) * (0.5f / kDigits) : 0.f,
+                       [&](int, int d) { return *reinterpret_cast<const i4*>(h.value(a, lane, t0 + 64 * n, d)); });
+  }
+}
+// The marked ones of a wave's steps 0 .. last, that of number i from key from + i * step on.
+template <int KS, int NT>
+TL_DEVICE void attn_marked(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnHead& h, const AttnMarks& marks, int from, int step, int last, int least) {
+  if (__builtin_expect(!__any(marks.bits), 1)) return;
+#pragma unroll 1
+  for (int i = 0; i <= last; ++i) {
+    const bool mine = (marks.bits >> (i >> marks.shift)) & 1u;
+    if (__any(mine)) attn_further<KS, NT>(s, a, h, from + i * step, from + i * step + 64 * NT > least, mine);
+  }
 }
 
 // A wave, a workgroup or a split knows of a row sum_t 2^(x_t) v_t = 2^M o and sum_t 2^(x_t) = 2^(M - E) sum.  Joins the
@@ -454,23 +579,16 @@ struct AttnTile {
     const i4* q = reinterpret_cast<const i4*>(p);
     return ONCE ? __builtin_nontemporal_load(q) : *q;
   }
-  TL_DEVICE void load_keys(const Q8AttnArgs& a, const int8_t* k0, const float* ks, const float* vs, int t0, int T) {
-    const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-    const int8_t* kp = k0 + (long long)(t0 + 16 * (row >> 2) + (row & 3)) * a.l.lanes;
-    c.load(a, ks, vs, t0, T);
+  TL_DEVICE void load_keys(const Q8AttnArgs& a, const AttnHead& h, int t0) {
+    c.load(a, h.ks, h.vs, threadIdx.x & 63, t0, h.T);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int d = 0; d < KS; ++d) {
-        const int at = 64 * d + 16 * g;
-        k[j][d] = codes(kp + 4 * j * a.l.lanes + (at < a.l.lanes ? at : 0));  // the query's digits are 0 from lanes on
-      }
+      for (int d = 0; d < KS; ++d) k[j][d] = codes(h.key(a, threadIdx.x & 63, t0, j, d));
   }
-  TL_DEVICE void load_values(const Q8AttnArgs& a, const int8_t* v0, int t0) {
-    const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-    const int8_t* vp = v0 + (long long)((t0 >> 4) + g) * (16 * a.l.lanes) + 16 * row;
+  TL_DEVICE void load_values(const Q8AttnArgs& a, const AttnHead& h, int t0) {
 #pragma unroll
-    for (int d = 0; d < 4 * KS; ++d) v[d] = codes(vp + (16 * d < a.l.lanes ? 256 * d : 0));
+    for (int d = 0; d < 4 * KS; ++d) v[d] = codes(h.value(a, threadIdx.x & 63, t0, d));
   }
 };
 
@@ -500,10 +618,7 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
   // few keys for so many workgroups: as many as have a tile for each wave, or one alone for up to two each
   const int tiles = (w.T + 63) / 64, nsplit = tiles <= 2 * kWaves ? 1 : min(a.nsplit, (tiles + kWaves - 1) / kWaves);
   if (split >= nsplit) return;
-  const int8_t* k = l.k + w.b * l.seq_codes + w.h * l.head_codes;
-  const int8_t* v = l.v + w.b * l.seq_codes + w.h * l.head_codes;
-  const float* ks = l.ks + w.b * l.seq_scales + w.h * l.head_scales;
-  const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
+  const AttnHead h(a, w);
   const int row = lane & 15, g = lane >> 4;
   const int step = 64 * kWaves * nsplit;
   int t0 = 64 * (split * kWaves + wave);
@@ -514,19 +629,23 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
     {
       float x[KS][16];
       const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0, w.rows, w.pos, w.T);
-      tile.load_keys(a, k, ks, vs, t0, w.T);
-      tile.load_values(a, v, t0);
+      tile.load_keys(a, h, t0);
+      tile.load_values(a, h, t0);
       attn_begin<KS>(s, x, a.l.head_size, seen);
     }
     const int least = attn_least(s.seen);
     auto key = [&](int, int j, int d) { return tile.k[j][d]; };
     auto val = [&](int, int d) { return tile.v[d]; };
-    for (; t0 + step < w.T; t0 += step) {
+    const int from = t0;
+    AttnMarks marks(w.T, step);
+    int i = 0;
+    for (; t0 + step < w.T; t0 += step, ++i) {
       AttnScales<1> c = tile.c;
-      attn_step<KS, 1>(s, a, c, t0, t0 + 64 > least, key, val, [&] { tile.load_keys(a, k, ks, vs, t0 + step, w.T); });
-      tile.load_values(a, v, t0 + step);
+      marks.mark(i, attn_step<KS, 1>(s, a, c, t0, t0 + 64 > least, key, val, [&] { tile.load_keys(a, h, t0 + step); }));
+      tile.load_values(a, h, t0 + step);
     }
-    attn_step<KS, 1>(s, a, tile.c, t0, t0 + 64 > least, key, val, [] {});
+    marks.mark(i, attn_step<KS, 1>(s, a, tile.c, t0, t0 + 64 > least, key, val, [] {}));
+    attn_marked<KS, 1>(s, a, h, marks, from, step, i, least);
   }
 
   // join the waves' rows
@@ -615,10 +734,7 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
   if (!attn_unit(a, blockIdx.x % pairs, a.tiles - 1 - blockIdx.x / pairs, 64, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int row = lane & 15, g = lane >> 4;
-  const int8_t* k = l.k + w.b * l.seq_codes + w.h * l.head_codes;
-  const int8_t* v = l.v + w.b * l.seq_codes + w.h * l.head_codes;
-  const float* ks = l.ks + w.b * l.seq_scales + w.h * l.head_scales;
-  const float* vs = l.vs + w.b * l.seq_scales + w.h * l.head_scales;
+  const AttnHead h(a, w);
 
   // wave i brings operands i, i + 4, ...; tiles behind the last key are not brought
   unsigned key_at[KS];
@@ -631,7 +747,7 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
     for (int f = 0; f < NT * KS; ++f) {
       const int n = f / KS, c = f % KS;  // operand (n, wave, c)
       if (t0 + 64 * n >= w.T) continue;
-      lds_bring(k + (long long)(t0 + 64 * n) * l.lanes, key_at[c], &kbuf[((n * 4 + wave) * KS + c) * 64]);
+      lds_bring(h.k + (long long)(t0 + 64 * n) * l.lanes, key_at[c], &kbuf[((n * 4 + wave) * KS + c) * 64]);
     }
   };
   auto values_in = [&](int t0) {
@@ -639,7 +755,7 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
     for (int f = 0; f < NT * KS; ++f) {
       const int n = f / KS, d = (f % KS) * 4 + wave;  // operand (n, d)
       if (t0 + 64 * n >= w.T || 16 * d >= l.lanes) continue;
-      lds_bring(v + (long long)(t0 + 64 * n) * l.lanes + 256 * d, value_at, &vbuf[(n * 4 * KS + d) * 64]);
+      lds_bring(h.v + (long long)(t0 + 64 * n) * l.lanes + 256 * d, value_at, &vbuf[(n * 4 * KS + d) * 64]);
     }
   };
 
@@ -653,9 +769,10 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
   }
   const int least = attn_least(s.seen);
   const int most = -attn_least(-s.seen);
+  AttnMarks marks(w.T, 64 * NT);
   for (int t0 = 0; t0 < w.T; t0 += 64 * NT) {
     AttnScales<NT> sc;
-    sc.load(a, ks, vs, t0, w.T);
+    sc.load(a, h.ks, h.vs, lane, t0, w.T);
     lds_wait();  // this chunk's keys are in, and every wave has left the last chunk's values
     values_in(t0);
     auto ready = [&] {
@@ -666,9 +783,11 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
       ready();
       continue;
     }
-    attn_step<KS, NT>(s, a, sc, t0, t0 + 64 * NT > least, [&](int n, int j, int c) { return kbuf[((n * 4 + j) * KS + c) * 64 + lane]; },
-                      [&](int n, int d) { return vbuf[(n * 4 * KS + d) * 64 + lane]; }, ready);
+    marks.mark(t0 / (64 * NT),
+               attn_step<KS, NT>(s, a, sc, t0, t0 + 64 * NT > least, [&](int n, int j, int c) { return kbuf[((n * 4 + j) * KS + c) * 64 + lane]; },
+                                 [&](int n, int d) { return vbuf[(n * 4 * KS + d) * 64 + lane]; }, ready));
   }
+  attn_marked<KS, NT>(s, a, h, marks, 0, 64 * NT, (w.T - 1) / (64 * NT), least);
   s.sum = rows_sum(s.sum);
   if (16 * wave + row >= w.nr) return;
   const AttnOut out(a, w, 16 * wave + row, s.M, s.sum, (float)s.E);

@@ -1,10 +1,17 @@
 """GPU: how near the attention over the int8 K/V cache comes to 64 bits, beside fp32 over the same codes.
 
-Limits go by an fp32 softmax in numpy over what the codes stand for: the root mean square over a call's rows of
-|got - exact| / |exact| (2-norms) is at most FACTOR times numpy's.  Both forms round each score to fp32 (1/2 ulp, or more
-for a sum of hs products), each weight (the exponential's ulp) and each sum.  The kernel adds an integer's rounding to the
-query, at most 2^-25 of 2 to 16 times its median component, and one to each weight: together no more than what numpy's own sum of hs
-products and its division add, so twice numpy's is what is expected at most, and half as much again is for the few rows of a call."""
+A limit has two parts, added as squares: what fp32 costs, and what the kernel's integers add.
+
+fp32: an fp32 softmax in numpy over what the codes stand for; the root mean square over a call's rows of
+|got - exact| / |exact| (2-norms), times FACTOR.  Both forms round each score to fp32 (half a step, or more for a sum of hs
+products), each weight (the exponential's step) and each sum.  The kernel's query adds at most half of 2^-24 of 2 to 16
+times its median component, no more than what a sum of hs products adds: twice numpy's is what is expected
+at most, and half as much again is for the few rows of a call.
+
+integers: a weight times its value block's scale is n 2^-23 of its step's largest w_t 2^e_t, and the scale at least half of
+2^e_t: off by up to half of 2^-22 of the largest weight times scale, 2^-22 / sqrt(12) in the mean.  A step has up to 256
+keys of about the same codes: sqrt(256) 2^-22 / sqrt(12) = 1.1e-6 of what the largest key itself adds to the row, and the
+row is no smaller than that where the values are of one size (where it is, the weights have more digits)."""
 import numpy as np
 import pytest
 
@@ -15,6 +22,7 @@ from test_q8_kv_gpu import Device, rows
 pytestmark = pytest.mark.gpu
 
 FACTOR = 3.0
+WEIGHTS = 16 * 2.0 ** -22 / 12 ** 0.5
 FORMS = [(4, 2, 1), (3, 2, 40), (2, 130, 70)]  # B, H, rows: one row a sequence, few rows, rows that fill the card
 
 
@@ -40,7 +48,7 @@ def off(got, want):
 
 
 def held(gpu, handle, ref, pos, q, what):
-    """The call's rows (some of them, where they are many) within FACTOR of fp32."""
+    """The call's rows (some of them, where they are many) within the limit."""
     B, nt, heads, hs = q.shape
     dev = Device(gpu, handle, ref)
     got = dev.attend(0, pos, None, q).reshape(q.shape)
@@ -48,7 +56,7 @@ def held(gpu, handle, ref, pos, q, what):
     want, _ = ref.attend(0, pos, [nt] * B, nt, q, heads // ref.H, some)
     want = want[:, some]
     mine, plain = off(got[:, some], want), off(fp32(ref, pos, q, some), want)
-    assert mine <= FACTOR * plain, f"{what}: {mine:.3g} off, fp32 {plain:.3g}"
+    assert mine <= np.hypot(FACTOR * plain, WEIGHTS), f"{what}: {mine:.3g} off, fp32 {plain:.3g}"
 
 
 @pytest.mark.parametrize("power", [0, 25, 30, 33, 36, -30, -36])
@@ -62,3 +70,49 @@ def test_scores_of_queries_and_keys_far_apart(gpu, handle, power, B, H, nt):
     q = (r.standard_normal((B, nt, H, hs)) * 10.0 ** power).astype(np.float32)
     ref.store(0, [0] * B, [S] * B, (k * 10.0 ** -power).astype(np.float32), v)
     held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q, f"10^{power}")
+
+
+@pytest.mark.parametrize("score,part,at", [(8, 0.05, [0]), (10, 0.01, [0]), (12, 0.01, [130]), (12, 0, [0]), (16, 0, [0]), (20, 0, [77]),
+                                           (12, 0, [0, 1, 2, 3]), (12, 0, [0, 64, 128, 192, 300])])
+@pytest.mark.parametrize("hs", [24, 64, 128, 160, 256])
+@pytest.mark.parametrize("B,H,nt", FORMS)
+def test_most_of_the_weight_on_keys_of_small_values(gpu, handle, score, part, at, hs, B, H, nt):
+    """Every row looks at one key, or a few, far more than at the others (a model's first token), and these have small
+    values or none: what is left of a row are the others, at weights down to 2^-30 of the largest."""
+    r = rng(nt + hs)
+    H = H if hs < 160 or H < 100 else 66
+    S = 600 if H < 100 else 400
+    k, v = r.standard_normal((B, S, H, hs)), r.standard_normal((B, S, H, hs))
+    q = r.standard_normal((B, nt, H, hs))
+    d = r.standard_normal((1, 1, H, hs))
+    d /= np.linalg.norm(d, axis=-1, keepdims=True)
+    q += (4 - (q * d).sum(-1, keepdims=True)) * d
+    k -= (k * d).sum(-1, keepdims=True) * d
+    k[:, at] = d * score * np.sqrt(hs) / 4
+    v[:, at] *= part
+    ref = Cache(B, 1, H, hs, S, 32, r)
+    ref.store(0, [0] * B, [S] * B, k.astype(np.float32), v.astype(np.float32))
+    held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q.astype(np.float32), f"{score}, values times {part}")
+
+
+@pytest.mark.parametrize("B,H,nt", FORMS[1:])
+def test_a_row_of_further_digits_leaves_its_neighbours(gpu, handle, B, H, nt):
+    """Rows whose weights need more digits do not change a bit of the rows beside them."""
+    r = rng(nt)
+    hs, S = 64, 300
+    k, v = r.standard_normal((B, S, H, hs)), r.standard_normal((B, S, H, hs))
+    q = r.standard_normal((B, nt, H, hs)).astype(np.float32)
+    v[:, 5] = 0
+    ref = Cache(B, 1, H, hs, S, 32, r)
+    ref.store(0, [0] * B, [S] * B, k.astype(np.float32), v.astype(np.float32))
+    dev = Device(gpu, handle, ref)
+    pos = [S - nt] * B
+    before = dev.attend(0, pos, None, q).reshape(q.shape)
+    some = [1, 18, nt - 2]
+    q[:, some] += (k[:, 5] / (k[:, 5] ** 2).sum(-1, keepdims=True) * 13 * np.sqrt(hs))[:, None].astype(np.float32)
+    got = dev.attend(0, pos, None, q).reshape(q.shape)
+    want, _ = ref.attend(0, pos, [nt] * B, nt, q, 1, some)
+    plain = off(fp32(ref, pos, q, some), want[:, some])
+    assert off(got[:, some], want[:, some]) <= np.hypot(FACTOR * plain, WEIGHTS)
+    rest = [i for i in range(nt) if i not in some]
+    np.testing.assert_array_equal(got[:, rest], before[:, rest])
