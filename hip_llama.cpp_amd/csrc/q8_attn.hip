@@ -9,10 +9,10 @@
 // three exact int8 products with int32 sums.  For the scores n = q / 2^e 0x7f7f7f, with 2^e the power of two over a
 // row's largest |q|: off by 2^-24 of that, as an fp32 number is.  For the values it is the softmax weight times the
 // value block's scale, w_t = 2^(x_t - m) sv_t, which is what has to be small beside the row's largest w: with
-// sv = f 2^e, 1/2 <= f < 1, the running maximum is taken of x_t + e_t, u_t = 2^(x_t + e_t - M) is at most 1 and
-// n_t = u_t f_t 0x7f7f7f.  The sum of the weights adds u_t 2^(E - e_t), E the row's largest e so far; value scales under
-// 2^(E - 40) count as that e with a smaller f, so that u_t cannot vanish where its weight does not; a row is so off by up
-// to 2^-64 of 127 of the largest value scale in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a
+// sv = f 2^e, 1/2 <= f < 1, and E the row's largest e so far, the running maximum M is taken of y_t = x_t + (e_t - E) (as
+// exact as x_t itself, whatever the values' size), u_t = 2^(y_t - M) is at most 1 and n_t = u_t f_t 0x7f7f7f.  The sum of
+// the weights adds u_t 2^(E - e_t); value scales under 2^(E - 40) count as that e with a smaller f, so that u_t cannot
+// vanish where its weight does not; a row is so off by up to 2^-64 of 127 of the largest value scale in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a
 // large weight elsewhere costs the step's own no digits; the steps are summed in fp32, in units of a power that follows
 // M only where it rises past 2^16 of it.  A large weight on a key of small values still costs its neighbours theirs (the
 // first token of a model, with nearly all of a row's weight and nothing in its values: without more, the row would be 4e-5 to 1e-1
@@ -102,7 +102,7 @@ struct AttnRows {
   int qe;        // their power of two, less kUnit
   float qn;      // 1, or NaN for a query that is not finite
   int seen;      // keys that the row sees
-  float M, sum;  // running maximum, sum of weights
+  float M, sum;  // running maximum (of scores and value exponents, these less E), sum of weights
   f4 o[4 * KS];  // sums over the values: dimensions 16 d + 4 (lane >> 4) .. + 3
   int E;         // largest value exponent that the row has seen
 
@@ -232,7 +232,7 @@ TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, At
   return true;
 }
 
-// Scores x_t + e_t of NT tiles of 64 keys, -inf for those that the row does not see, whose factors become 0.
+// Scores x_t + (e_t - E) of NT tiles of 64 keys, -inf for those that the row does not see, whose factors become 0.
 // key: (tile, 16-key step, 64-dimension step) -> sixteen codes.
 template <int KS, int NT, class Key>
 TL_DEVICE void attn_scores(f4 (&x)[NT][4], AttnScales<NT>& c, const AttnRows<KS>& s, const Q8AttnArgs& a, bool edge, int left, Key key) {
@@ -261,7 +261,7 @@ TL_DEVICE void attn_scores(f4 (&x)[NT][4], AttnScales<NT>& c, const AttnRows<KS>
         const int n = (u - 1) / 4, j = (u - 1) & 3;
         if (j == 0) {
           c1 = __builtin_ldexpf(a.c0 * c.sk[n], s.qe) * s.qn;
-          ce = (float)c.e[n];
+          ce = (float)(c.e[n] - s.E);
         }
         const i4(&r)[3] = acc[(u - 1) & 1];
 #pragma unroll
@@ -366,13 +366,14 @@ TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT
     top = max((int)r.x, (int)r.y);
     grow = top - s.E;
     s.E = top;
+    s.M -= (float)grow;  // kNone stays
   }
   c.factors(s.E);
   f4 x[NT][4];
   attn_scores<KS, NT>(x, c, s, a, edge, left, key);
   const float m = attn_most<NT>(x);  // of this step alone: it sets the size that the step's weights are rounded to
   // Rare behind the first step (four prompts of 2048 tokens, 32 heads of 128: 272 us; scaled in each step 276).
-  const float M = m - kLag > s.M ? m : s.M;
+  const float M = m - kLag > s.M ? __builtin_ceilf(m) : s.M;  // whole, so that it moves by grow without a rounding
   if (__any(M != s.M || grow)) {
     const float alpha = __builtin_amdgcn_exp2f(s.M - M);
 #pragma unroll
@@ -503,27 +504,28 @@ TL_DEVICE void attn_marked(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnHead&
   }
 }
 
-// A wave, a workgroup or a split knows of a row sum_t 2^(x_t) v_t = 2^M o and sum_t 2^(x_t) = 2^(M - E) sum.  Joins the
+// A wave, a workgroup or a split knows of a row sum_t 2^(x_t) v_t = 2^(M + E) o and sum_t 2^(x_t) = 2^M sum.  Joins the
 // first n of N such parts, st = (M, sum, E), to one.
 template <int N>
 TL_DEVICE void parts_join(const f4 (&x)[N], const f4 (&st)[N], int n, f4& o, float& M, float& sum, float& E) {
-  float m = M, top = E;
+  float top = E;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (i >= n) continue;
-    m = fmaxf(m, st[i].x);
-    top = fmaxf(top, st[i].z);
-  }
-  auto weight = [&](float M1, float sum1, float E1) { return sum1 == 0.f ? 0.f : __builtin_amdgcn_exp2f((M1 - m) + (top - E1)) * sum1; };
-  sum = weight(M, sum, E);
-  const float w = __builtin_amdgcn_exp2f(M - m);
+  for (int i = 0; i < N; ++i)
+    if (i < n) top = fmaxf(top, st[i].z);
+  float m = M + (E - top);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n) m = fmaxf(m, st[i].x + (st[i].z - top));
+  auto weight = [&](float M1, float sum1) { return sum1 == 0.f ? 0.f : __builtin_amdgcn_exp2f(M1 - m) * sum1; };
+  sum = weight(M, sum);
+  const float w = __builtin_amdgcn_exp2f(M + (E - top) - m);
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= w;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (i >= n) continue;
-    sum += weight(st[i].x, st[i].y, st[i].z);
-    const float wi = __builtin_amdgcn_exp2f(st[i].x - m);
+    sum += weight(st[i].x, st[i].y);
+    const float wi = __builtin_amdgcn_exp2f(st[i].x + (st[i].z - top) - m);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], wi, o[e]);
   }

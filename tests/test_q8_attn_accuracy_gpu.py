@@ -116,3 +116,18 @@ def test_a_row_of_further_digits_leaves_its_neighbours(gpu, handle, B, H, nt):
     assert off(got[:, some], want[:, some]) <= np.hypot(FACTOR * plain, WEIGHTS)
     rest = [i for i in range(nt) if i not in some]
     np.testing.assert_array_equal(got[:, rest], before[:, rest])
+
+
+@pytest.mark.parametrize("first,rest", [(1e-30, 1e-30), (1e30, 1e30), (1e-30, 1e-28), (1e-37, 1e30), (1e30, 1e-5)])
+@pytest.mark.parametrize("B,H,nt", FORMS)
+def test_values_of_any_size(gpu, handle, first, rest, B, H, nt):
+    """Small and large values, and values whose size changes on the way, cost the weights no bits."""
+    r = rng(nt + int(np.log10(first * rest)) + 100)
+    hs, S = 64, 500
+    ref = Cache(B, 1, H, hs, S, 32, r)
+    k, v = rows(r, B, S, H, hs), rows(r, B, S, H, hs)
+    v[:, :300] *= np.float32(first)
+    v[:, 300:] *= np.float32(rest)
+    q = r.standard_normal((B, nt, H, hs)).astype(np.float32)
+    ref.store(0, [0] * B, [S] * B, k, v)
+    held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q, f"{first} then {rest}")
