@@ -7,7 +7,8 @@
 // (balanced digits: those of n + 0x8080, the lower two less 0x80), so
 //   sum n c = 2^16 sum d2 c + (2^8 sum d1 c + sum d0 c),
 // three exact int8 products with int32 sums.  For the scores n = q / 2^e 0x7f7f7f, with 2^e the power of two over a
-// row's largest |q|: off by 2^-24 of that, as an fp32 number is.  For the values it is the softmax weight times the
+// row's largest |q|: off by 2^-24 of that, as an fp32 number is; rows whose largest is far above the others, which would be
+// left few of these bits, take their keys again with three digits more.  For the values it is the softmax weight times the
 // value block's scale, w_t = 2^(x_t - m) sv_t, which is what has to be small beside the row's largest w: with
 // sv = f 2^e, 1/2 <= f < 1, and E the row's largest e so far, the running maximum M is taken of y_t = x_t + (e_t - E) (as
 // exact as x_t itself, whatever the values' size), u_t = 2^(y_t - M) is at most 1 and n_t = u_t f_t 0x7f7f7f.  The sum of
@@ -115,6 +116,25 @@ struct AttnRows {
   }
 };
 
+struct AttnUnit {  // what a workgroup works on
+  int b, h, r0, rows, nr, T;
+  long long pos;
+};
+// Row tile `tile` of R rows of pair (b, h); false if the sequence has no such rows.
+TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, AttnUnit& w) {
+  w.h = pair % a.l.heads;
+  w.b = pair / a.l.heads;
+  int count;
+  q8kv_start(a.call, w.b, w.pos, count);
+  w.rows = count * a.mul;
+  w.r0 = tile * R;
+  if (w.r0 >= w.rows) return false;
+  w.nr = min(R, w.rows - w.r0);
+  const long long first = w.pos + w.r0 / a.mul, last = w.pos + (w.r0 + w.nr - 1) / a.mul;
+  w.T = first >= a.l.seq_len ? 0 : (int)max(0LL, min(last + 1, (long long)a.l.seq_len));
+  return true;
+}
+
 // This lane's part of row r0 + (lane & 15) of the `rows` of (b, h), and the keys that the row sees.  A row behind the
 // last is the last one again; it sees what the tile sees and is never stored.  Every load is made, from inside the row, so that
 // none is waited for before the next is asked for.
@@ -143,18 +163,31 @@ TL_DEVICE int attn_query(float (&x)[KS][16], const Q8AttnArgs& a, int b, int h, 
   return r0 + (lane & 15) >= rows ? T : p >= 0 && p < a.l.seq_len ? (int)p + 1 : 0;
 }
 
-// The query's digits.
+// 0 behind the head's end.
 template <int KS>
-TL_DEVICE void attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen) {
+TL_DEVICE void attn_clip(float (&x)[KS][16], int hs) {
+  if (hs >= 64 * KS) return;
+  const int left = hs - 16 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (64 * k + e >= left) x[k][e] = 0.f;
+}
+
+// Three more digits of the query, for rows that need them: 1 / 0x7f7f7f of the others'.
+template <int KS, bool WIDE>
+struct AttnMore {
+  i4 q[3][WIDE ? KS : 1];
+};
+
+// The query's digits.  True if they are too few for the row: where a few components are so much larger than the rest that
+// these have few of the 24 bits.  Goes by the mean of every other eight components, none taken for more than 2^-4 of the
+// largest number: under 3/8 of that where the largest component is past some 34 times the width of the others' distribution.
+template <int KS>
+TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen) {
   s.seen = seen;
-  if (hs < 64 * KS) {
-    const int left = hs - 16 * ((threadIdx.x & 63) >> 4);
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (64 * k + e >= left) x[k][e] = 0.f;
-  }
+  attn_clip<KS>(x, hs);
   unsigned top = 0;
 #pragma unroll
   for (int k = 0; k < KS; ++k)
@@ -164,19 +197,26 @@ TL_DEVICE void attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
   s.qn = top < 0x7f800000u ? 1.f : __builtin_nanf("");
   const int qe = top < 0x7f800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
   s.qe = qe - kUnit;
+  constexpr float most = kDigits / 16.f;
+  float size = 0.f;
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       unsigned n[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) n[c] = (unsigned)(int)rintf(__builtin_ldexpf(x[k][4 * e + c], -qe) * kDigits) + 0x8080u;
+      for (int c = 0; c < 4; ++c) {
+        const float y = __builtin_ldexpf(x[k][4 * e + c], -qe) * kDigits;
+        if (e < 2) size += fminf(fabsf(y), most);
+        n[c] = (unsigned)(int)rintf(y) + 0x8080u;
+      }
       int p0, p1, p2;
       digits4(n, p0, p1, p2);
       s.q[0][k][e] = p0;
       s.q[1][k][e] = p1;
       s.q[2][k][e] = p2;
     }
+  return rows_sum(size) < 0.375f * most * (float)((hs >> 4) * 8 + min(hs & 15, 8)) && top > 0u && top < 0x7f800000u;
 }
 
 // Scales of this lane's sixteen keys in each of NT tiles of 64 from t0 on; behind the last key those of its block.
@@ -213,33 +253,17 @@ struct AttnScales {
   }
 };
 
-struct AttnUnit {  // what a workgroup works on
-  int b, h, r0, rows, nr, T;
-  long long pos;
-};
-// Row tile `tile` of R rows of pair (b, h); false if the sequence has no such rows.
-TL_DEVICE bool attn_unit(const Q8AttnArgs& a, unsigned pair, int tile, int R, AttnUnit& w) {
-  w.h = pair % a.l.heads;
-  w.b = pair / a.l.heads;
-  int count;
-  q8kv_start(a.call, w.b, w.pos, count);
-  w.rows = count * a.mul;
-  w.r0 = tile * R;
-  if (w.r0 >= w.rows) return false;
-  w.nr = min(R, w.rows - w.r0);
-  const long long first = w.pos + w.r0 / a.mul, last = w.pos + (w.r0 + w.nr - 1) / a.mul;
-  w.T = first >= a.l.seq_len ? 0 : (int)max(0LL, min(last + 1, (long long)a.l.seq_len));
-  return true;
-}
-
 // Scores x_t + (e_t - E) of NT tiles of 64 keys, -inf for those that the row does not see, whose factors become 0.
 // key: (tile, 16-key step, 64-dimension step) -> sixteen codes.
-template <int KS, int NT, class Key>
-TL_DEVICE void attn_scores(f4 (&x)[NT][4], AttnScales<NT>& c, const AttnRows<KS>& s, const Q8AttnArgs& a, bool edge, int left, Key key) {
+template <int KS, int NT, bool WIDE, class Key>
+TL_DEVICE void attn_scores(f4 (&x)[NT][4], AttnScales<NT>& c, const AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, bool edge, int left,
+                           Key key) {
   // Each turn asks for the next one's operands, starts this one's products and finishes the last one's, so that neither
   // LDS nor the matrix pipe is waited for.
   {
-    i4 k[2][KS], acc[2][3];
+    constexpr int Z = WIDE ? 6 : 3;
+    i4 k[2][KS], acc[2][Z];
+    auto digits = [&](int z, int d) { return z < 3 ? s.q[z % 3][d] : more.q[z % 3][WIDE ? d : 0]; };
     float c1 = 0.f, ce = 0.f;
 #pragma unroll
     for (int d = 0; d < KS; ++d) k[0][d] = key(0, 0, d);
@@ -251,11 +275,11 @@ TL_DEVICE void attn_scores(f4 (&x)[NT][4], AttnScales<NT>& c, const AttnRows<KS>
       }
       if (u < 4 * NT) {
 #pragma unroll
-        for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(k[u & 1][0], s.q[z][0], i4{0, 0, 0, 0});
+        for (int z = 0; z < Z; ++z) acc[u & 1][z] = mfma(k[u & 1][0], digits(z, 0), i4{0, 0, 0, 0});
 #pragma unroll
         for (int d = 1; d < KS; ++d)
 #pragma unroll
-          for (int z = 0; z < 3; ++z) acc[u & 1][z] = mfma(k[u & 1][d], s.q[z][d], acc[u & 1][z]);
+          for (int z = 0; z < Z; ++z) acc[u & 1][z] = mfma(k[u & 1][d], digits(z, d), acc[u & 1][z]);
       }
       if (u > 0) {
         const int n = (u - 1) / 4, j = (u - 1) & 3;
@@ -263,10 +287,13 @@ TL_DEVICE void attn_scores(f4 (&x)[NT][4], AttnScales<NT>& c, const AttnRows<KS>
           c1 = __builtin_ldexpf(a.c0 * c.sk[n], s.qe) * s.qn;
           ce = (float)(c.e[n] - s.E);
         }
-        const i4(&r)[3] = acc[(u - 1) & 1];
+        const i4(&r)[Z] = acc[(u - 1) & 1];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[n][j][i] = fmaf((float)r[2][i], 65536.f * c1, fmaf((float)((r[1][i] << 8) + r[0][i]), c1, ce));
+        for (int i = 0; i < 4; ++i) {
+          float y = fmaf((float)r[2][i], 65536.f * c1, fmaf((float)((r[1][i] << 8) + r[0][i]), c1, ce));
+          if constexpr (WIDE) y = fmaf(fmaf((float)r[5][i], 65536.f, (float)((r[4][i] << 8) + r[3][i])), c1 * (1.f / kDigits), y);
+          x[n][j][i] = y;
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -350,8 +377,8 @@ struct AttnHead {
 
 // One step of NT tiles of 64 keys from t0 on; key and val as above.  ready() runs between the two products.  The rows of
 // the wave whose weights need further digits, as bits.
-template <int KS, int NT, class Key, class Val, class Ready>
-TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
+template <int KS, int NT, bool WIDE, class Key, class Val, class Ready>
+TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
   constexpr int DT = 4 * KS;
   const int g = (threadIdx.x & 63) >> 4;
   const int left = s.seen - t0 - 16 * g;  // keys of this lane's first tile and behind it that the row sees
@@ -370,7 +397,7 @@ TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const Q8AttnArgs& a, AttnScales<NT
   }
   c.factors(s.E);
   f4 x[NT][4];
-  attn_scores<KS, NT>(x, c, s, a, edge, left, key);
+  attn_scores<KS, NT>(x, c, s, more, a, edge, left, key);
   const float m = attn_most<NT>(x);  // of this step alone: it sets the size that the step's weights are rounded to
   // Rare behind the first step (four prompts of 2048 tokens, 32 heads of 128: 272 us; scaled in each step 276).
   const float M = m - kLag > s.M ? __builtin_ceilf(m) : s.M;  // whole, so that it moves by grow without a rounding
@@ -451,8 +478,8 @@ struct AttnMarks {
 // A row needs it where one key has far more weight than others and next to nothing in its values (a model's first token),
 // in the steps that hold such a key.  Its operands are read again when all keys are through, and taken tile by tile: in the
 // loop itself the registers would be short.
-template <int KS, int NT>
-TL_DEVICE void attn_further(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnHead& h, int t0, bool edge, bool mine) {
+template <int KS, int NT, bool WIDE>
+TL_DEVICE void attn_further(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, const AttnHead& h, int t0, bool edge, bool mine) {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // addresses are made here, not ahead and kept in registers
   const int left = s.seen - t0 - 16 * (lane >> 4), tiles = min(NT, (h.T - t0 + 63) / 64);
@@ -462,7 +489,7 @@ TL_DEVICE void attn_further(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnHead
     c.load(a, h.ks, h.vs, lane, t0 + 64 * n, h.T);
     c.exponents(edge, left - 64 * n);
     c.factors(s.E);
-    attn_scores<KS, 1>(x, c, s, a, edge, left - 64 * n, [&](int, int j, int d) { return *reinterpret_cast<const i4*>(h.key(a, lane, t0 + 64 * n, j, d)); });
+    attn_scores<KS, 1>(x, c, s, more, a, edge, left - 64 * n, [&](int, int j, int d) { return *reinterpret_cast<const i4*>(h.key(a, lane, t0 + 64 * n, j, d)); });
   };
   float m = kNone;  // the step's
 #pragma unroll 1
@@ -494,14 +521,60 @@ TL_DEVICE void attn_further(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnHead
   }
 }
 // The marked ones of a wave's steps 0 .. last, that of number i from key from + i * step on.
-template <int KS, int NT>
-TL_DEVICE void attn_marked(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnHead& h, const AttnMarks& marks, int from, int step, int last, int least) {
+template <int KS, int NT, bool WIDE>
+TL_DEVICE void attn_marked(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, const AttnHead& h, const AttnMarks& marks, int from, int step, int last, int least) {
   if (__builtin_expect(!__any(marks.bits), 1)) return;
 #pragma unroll 1
   for (int i = 0; i <= last; ++i) {
     const bool mine = (marks.bits >> (i >> marks.shift)) & 1u;
-    if (__any(mine)) attn_further<KS, NT>(s, a, h, from + i * step, from + i * step + 64 * NT > least, mine);
+    if (__any(mine)) attn_further<KS, NT>(s, more, a, h, from + i * step, from + i * step + 64 * NT > least, mine);
   }
+}
+
+// These, from the query's values again.
+template <int KS>
+TL_DEVICE AttnMore<KS, true> attn_more(const AttnRows<KS>& s, const Q8AttnArgs& a, const AttnUnit& w, int r0, bool mine) {
+  float x[KS][16];
+  (void)attn_query<KS>(x, a, w.b, w.h, r0, w.rows, w.pos, w.T);
+  attn_clip<KS>(x, a.l.head_size);
+  AttnMore<KS, true> more;
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      unsigned n[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float y = __builtin_ldexpf(x[k][4 * e + c], -(s.qe + kUnit));
+        n[c] = (unsigned)(int)rintf(fmaf(y, kDigits, -rintf(y * kDigits)) * kDigits) + 0x8080u;  // at most 3/4 is left: two roundings
+      }
+      int p0, p1, p2;
+      digits4(n, p0, p1, p2);
+      more.q[0][k][e] = mine ? p0 : 0;  // the others' rows stay as they are without
+      more.q[1][k][e] = mine ? p1 : 0;
+      more.q[2][k][e] = mine ? p2 : 0;
+    }
+  return more;
+}
+
+// A wave's keys, its steps of 64 from key `from` on `step` apart, with six digits of the queries that want them (`mine`).
+// Rare, and plain.
+template <int KS>
+TL_DEVICE void attn_wide(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnUnit& w, const AttnHead& h, int r0, bool mine, int from, int step, int least) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // as above
+  const AttnMore<KS, true> more = attn_more<KS>(s, a, w, r0, mine);
+  AttnMarks marks(h.T, step);
+  s.none();
+  int i = 0;
+#pragma unroll 1
+  for (int t0 = from; t0 < h.T; t0 += step, ++i) {
+    AttnScales<1> c;
+    c.load(a, h.ks, h.vs, lane, t0, h.T);
+    marks.mark(i, attn_step<KS, 1>(s, more, a, c, t0, t0 + 64 > least, [&](int, int j, int d) { return *reinterpret_cast<const i4*>(h.key(a, lane, t0, j, d)); },
+                                   [&](int, int d) { return *reinterpret_cast<const i4*>(h.value(a, lane, t0, d)); }, [] {}));
+  }
+  attn_marked<KS, 1>(s, more, a, h, marks, from, step, i - 1, least);
 }
 
 // A wave, a workgroup or a split knows of a row sum_t 2^(x_t) v_t = 2^(M + E) o and sum_t 2^(x_t) = 2^M sum.  Joins the
@@ -628,26 +701,32 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
   s.none();
   if (t0 < w.T) {
     AttnTile<KS, ONCE> tile;
+    bool more;
     {
       float x[KS][16];
       const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0, w.rows, w.pos, w.T);
       tile.load_keys(a, h, t0);
       tile.load_values(a, h, t0);
-      attn_begin<KS>(s, x, a.l.head_size, seen);
+      more = attn_begin<KS>(s, x, a.l.head_size, seen);
     }
     const int least = attn_least(s.seen);
-    auto key = [&](int, int j, int d) { return tile.k[j][d]; };
-    auto val = [&](int, int d) { return tile.v[d]; };
-    const int from = t0;
-    AttnMarks marks(w.T, step);
-    int i = 0;
-    for (; t0 + step < w.T; t0 += step, ++i) {
-      AttnScales<1> c = tile.c;
-      marks.mark(i, attn_step<KS, 1>(s, a, c, t0, t0 + 64 > least, key, val, [&] { tile.load_keys(a, h, t0 + step); }));
-      tile.load_values(a, h, t0 + step);
+    if (__builtin_expect(__any(more), 0)) {
+      attn_wide<KS>(s, a, w, h, w.r0, more, t0, step, least);
+    } else {
+      const AttnMore<KS, false> none{};
+      auto key = [&](int, int j, int d) { return tile.k[j][d]; };
+      auto val = [&](int, int d) { return tile.v[d]; };
+      const int from = t0;
+      AttnMarks marks(w.T, step);
+      int i = 0;
+      for (; t0 + step < w.T; t0 += step, ++i) {
+        AttnScales<1> c = tile.c;
+        marks.mark(i, attn_step<KS, 1>(s, none, a, c, t0, t0 + 64 > least, key, val, [&] { tile.load_keys(a, h, t0 + step); }));
+        tile.load_values(a, h, t0 + step);
+      }
+      marks.mark(i, attn_step<KS, 1>(s, none, a, tile.c, t0, t0 + 64 > least, key, val, [] {}));
+      attn_marked<KS, 1>(s, none, a, h, marks, from, step, i, least);
     }
-    marks.mark(i, attn_step<KS, 1>(s, a, tile.c, t0, t0 + 64 > least, key, val, [] {}));
-    attn_marked<KS, 1>(s, a, h, marks, from, step, i, least);
   }
 
   // join the waves' rows
@@ -726,7 +805,7 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
 // holds under this load.  Two tiles a step leave room for three waves on a SIMD (343 us, four tiles and two waves 352, on
 // one card), heads of 64 fit three with four.
 template <int KS, int NT>
-__global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_many(Q8AttnArgs a) {
+__global__ void __launch_bounds__(256, KS < 3 ? 3 : 2) k_q8_attn_many(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp
   __shared__ __attribute__((aligned(1024))) i4 kbuf[NT * 4 * KS * 64];
   __shared__ __attribute__((aligned(1024))) i4 vbuf[NT * 4 * KS * 64];
@@ -764,11 +843,13 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
   if (w.T > 0) keys_in(0);
   AttnRows<KS> s;
   s.none();
+  bool more;
   {
     float x[KS][16];
     const int seen = attn_query<KS>(x, a, w.b, w.h, w.r0 + 16 * wave, w.rows, w.pos, w.T);
-    attn_begin<KS>(s, x, a.l.head_size, seen);
+    more = attn_begin<KS>(s, x, a.l.head_size, seen);
   }
+  const AttnMore<KS, false> none{};
   const int least = attn_least(s.seen);
   const int most = -attn_least(-s.seen);
   AttnMarks marks(w.T, 64 * NT);
@@ -786,16 +867,23 @@ __global__ void __launch_bounds__(256, KS < 3 ? 3 : KS < 4 ? 2 : 1) k_q8_attn_ma
       continue;
     }
     marks.mark(t0 / (64 * NT),
-               attn_step<KS, NT>(s, a, sc, t0, t0 + 64 * NT > least, [&](int n, int j, int c) { return kbuf[((n * 4 + j) * KS + c) * 64 + lane]; },
+               attn_step<KS, NT>(s, none, a, sc, t0, t0 + 64 * NT > least, [&](int n, int j, int c) { return kbuf[((n * 4 + j) * KS + c) * 64 + lane]; },
                                  [&](int n, int d) { return vbuf[(n * 4 * KS + d) * 64 + lane]; }, ready));
   }
-  attn_marked<KS, NT>(s, a, h, marks, 0, 64 * NT, (w.T - 1) / (64 * NT), least);
-  s.sum = rows_sum(s.sum);
-  if (16 * wave + row >= w.nr) return;
-  const AttnOut out(a, w, 16 * wave + row, s.M, s.sum, (float)s.E);
+  attn_marked<KS, NT>(s, none, a, h, marks, 0, 64 * NT, (w.T - 1) / (64 * NT), least);
+  auto leave = [&](bool mine) {
+    const float sum = rows_sum(s.sum);
+    if (16 * wave + row >= w.nr || !mine) return;
+    const AttnOut out(a, w, 16 * wave + row, s.M, sum, (float)s.E);
 #pragma unroll
-  for (int d = 0; d < 4 * KS; ++d)
-    if (16 * d + 4 * g < l.head_size) out.store(a, 16 * d + 4 * g, s.o[d]);
+    for (int d = 0; d < 4 * KS; ++d)
+      if (16 * d + 4 * g < l.head_size) out.store(a, 16 * d + 4 * g, s.o[d]);
+  };
+  leave(!more);
+  if (__builtin_expect(__any(more), 0)) {
+    attn_wide<KS>(s, a, w, h, w.r0 + 16 * wave, true, 0, 64, least);
+    leave(more);
+  }
 }
 
 constexpr int kAttnUnits = 256;  // row tiles that fill the card by themselves: one for each CU

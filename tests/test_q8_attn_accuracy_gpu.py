@@ -131,3 +131,42 @@ def test_values_of_any_size(gpu, handle, first, rest, B, H, nt):
     q = r.standard_normal((B, nt, H, hs)).astype(np.float32)
     ref.store(0, [0] * B, [S] * B, k, v)
     held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q, f"{first} then {rest}")
+
+
+@pytest.mark.parametrize("size,count,keys", [(20, 1, 0), (50, 1, 0), (50, 1, 1), (50, 3, 0), (1000, 1, 0), (1000, 1, 0.02), (1e5, 1, 0), (1e6, 2, 0)])
+@pytest.mark.parametrize("hs", [64, 128, 192, 256])
+@pytest.mark.parametrize("B,H,nt", FORMS)
+def test_queries_of_a_few_large_components(gpu, handle, size, count, keys, hs, B, H, nt):
+    """Components far larger than the rest, where the keys have little or nothing, take none of the others' bits."""
+    r = rng(nt + hs + count)
+    H = H if hs < 160 or H < 100 else 66
+    S = 300
+    k, v = r.standard_normal((B, S, H, hs)), r.standard_normal((B, S, H, hs))
+    q = r.standard_normal((B, nt, H, hs))
+    large = r.choice(hs, count, replace=False)
+    q[..., large] = size
+    k[..., large] *= keys
+    ref = Cache(B, 1, H, hs, S, 32, r)
+    ref.store(0, [0] * B, [S] * B, k.astype(np.float32), v.astype(np.float32))
+    held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q.astype(np.float32), f"{count} of {size}, keys times {keys}")
+
+
+@pytest.mark.parametrize("B,H,nt", FORMS[1:])
+def test_a_row_of_large_components_leaves_its_neighbours(gpu, handle, B, H, nt):
+    """Rows whose queries need more digits do not change a bit of the rows beside them."""
+    r = rng(nt + 1)
+    hs, S = 128, 300
+    k, v = r.standard_normal((B, S, H, hs)), r.standard_normal((B, S, H, hs))
+    q = r.standard_normal((B, nt, H, hs)).astype(np.float32)
+    k[..., 7] = 0
+    ref = Cache(B, 1, H, hs, S, 32, r)
+    ref.store(0, [0] * B, [S] * B, k.astype(np.float32), v.astype(np.float32))
+    dev = Device(gpu, handle, ref)
+    pos = [S - nt] * B
+    before = dev.attend(0, pos, None, q).reshape(q.shape)
+    some = [1, 18, nt - 2]
+    q[:, some, :, 7] = 1e4
+    got = dev.attend(0, pos, None, q).reshape(q.shape)
+    rest = [i for i in range(nt) if i not in some]
+    np.testing.assert_array_equal(got[:, rest], before[:, rest])
+    assert off(got[:, some], before[:, some].astype(np.float64)) < 1e-5  # the keys have nothing there
