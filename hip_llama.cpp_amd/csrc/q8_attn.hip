@@ -633,10 +633,10 @@ struct AttnOut {
 
 // 16 bytes a lane from memory, at `from` + the lane's offset, to LDS, at `to` + 16 * lane; lds_wait: everybody's have
 // arrived.  Written out, because with the builtin the compiler waits for every load under way before the next read of any
-// LDS.  m0 has no other use in a kernel that calls this.
+// LDS.
 TL_DEVICE void lds_bring(const int8_t* from, unsigned offset, i4* to) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)to);
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(at) : "memory", "m0");
 }
 TL_DEVICE void lds_wait() {
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
