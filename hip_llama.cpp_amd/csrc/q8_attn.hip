@@ -636,7 +636,7 @@ struct AttnOut {
 // LDS.
 TL_DEVICE void lds_bring(const int8_t* from, unsigned offset, i4* to) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)to);
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(at) : "memory", "m0");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "{m0}"(at) : "memory");
 }
 TL_DEVICE void lds_wait() {
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
