@@ -510,7 +510,9 @@ extern "C" int thallama_memcpy_d2d(void* dst, const void* src, size_t bytes) {
 }
 extern "C" int thallama_memset(void* dst, int value, size_t bytes) {
   tl::ApiLock lock(tl::api_mu());
-  return (int)hipMemset(dst, value, bytes);
+  // hipMemset may return before the fill is done, and streams made by thablasCreate do not wait for the legacy one
+  const hipError_t e = hipMemset(dst, value, bytes);
+  return (int)(e == hipSuccess ? hipStreamSynchronize(nullptr) : e);
 }
 extern "C" int thallama_sync(void) {
   tl::ApiLock lock(tl::api_mu());

@@ -74,7 +74,9 @@ size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batches, int n_to
 // A decode step is n_tokens = 1 after its token's store, a prompt's chunk n_tokens > 1.
 // A row at a position outside 0 .. seq_len - 1 sees no key: zeros.  Rows from n_d[b] on are left as they were.
 // q and out are [n_batches][n_tokens][n_heads * head_size] and do not overlap.  work (16-byte aligned) is zeroed once,
-// before its first call (thallama_memset), and then left to these calls, of any shape: each leaves it ready for the next.  It
+// before its first call, and then left to these calls, of any shape: each leaves it ready for the next.  The zeroing is done
+// before that call's kernel runs: by thallama_memset, which waits for it, or by hipMemsetAsync on handle->calc_stream, outside
+// any capture (a plain hipMemset is not ordered before that stream).  It
 // belongs to a call until its kernel has run: calls that may run at once, captured ones among them, have one each.  A
 // call during which pos_d or n_d change leaves it to be zeroed again.
 thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, const Q8KVCache* c, int layer, int n_batches,

@@ -186,7 +186,7 @@ int thallama_free(void* p);
 int thallama_memcpy_h2d(void* dst, const void* src, size_t bytes);
 int thallama_memcpy_d2h(void* dst, const void* src, size_t bytes);
 int thallama_memcpy_d2d(void* dst, const void* src, size_t bytes);
-int thallama_memset(void* dst, int value, size_t bytes);
+int thallama_memset(void* dst, int value, size_t bytes); /* done when it returns */
 int thallama_sync(void);
 const char* thallama_last_error(void);
 
