@@ -438,6 +438,7 @@ extern "C" int thallama_decoder_create(thallama_decoder** out, const Config* cfg
     TL_TRY(hipMalloc(&d->pkgran, sizeof(unsigned long long) * nk));
     TL_TRY(hipMemset(d->pkgran, 0, sizeof(unsigned long long) * nk));
   }
+  TL_TRY(hipStreamSynchronize(nullptr));  // the fills above return before they are done, and d->stream does not wait for them
   *out = d;
   return 0;
 }
