@@ -173,6 +173,7 @@ struct thallama_decoder {
   bool use_graph = false;
   bool profile = false;
   bool persist = true;          // requested (THALLAMA_OPT_PERSISTENT)
+  int pcoop = -1;               // persistent launches are cooperative (-1: not asked yet)
   bool pfault = false;          // test hook: the next persistent launch loses block 0
   bool pasync = false;          // an asynchronous greedy call ran persistent launches not yet checked
   // [lc]: lc = 1 is the persistent step's long-context instantiation (persistent_long_ctx)
@@ -397,7 +398,6 @@ extern "C" int thallama_decoder_create(thallama_decoder** out, const Config* cfg
       why = "batch > 8";
     }
     if (!d->pok && why) d->pwhy = why;
-    if (d->pok) (void)tl::persistent_cooperative();  // found out here: a launch may be captured
   }
   if (!d->mpart_d) {  // split-K scratch of the matrix-core GEMV (batch 1: prefill's short chunks)
     const size_t nblk = (size_t)tl::mfma_target_blocks();
@@ -839,6 +839,7 @@ static int enqueue_persistent(thallama_decoder* d, bool argmax, int lc) {
   p.err = d->psync + d->psync_zero; p.seq = p.err + 1; p.bmax = d->pbmax;
   p.argmax = argmax ? 1 : 0;
   p.long_ctx = lc;
+  p.coop = d->pcoop > 0;
   p.trace = d->ptrace;
   p.fault = d->pfault ? 1 : 0;
   d->pfault = false;  // one-shot (a captured graph keeps it; the give-up drops the graph)
@@ -981,6 +982,11 @@ static int upload_tok_pos(thallama_decoder* d, const int* token_h, const int* po
   return 0;
 }
 
+// Before a decoder's first persistent step, and before that is captured: can it be a cooperative launch?
+static void ask_cooperative(thallama_decoder* d) {
+  if (use_persist(d) && d->pcoop < 0) d->pcoop = tl::persistent_cooperative_take();
+}
+
 static int decoder_forward_once(thallama_decoder* d, const int* token_h, const int* pos_h, float* logits_h);
 
 // Ends the capture begun on d->stream (also after an enqueue error `e`, so the stream leaves capture
@@ -1033,6 +1039,7 @@ static int decoder_forward_once(thallama_decoder* d, const int* token_h, const i
   if (!d || !token_h || !pos_h) return (int)hipErrorInvalidValue;
   int r = upload_tok_pos(d, token_h, pos_h);
   if (r) return r;
+  ask_cooperative(d);
   if (d->use_graph && !d->profile) {  // the step (~160 launches at batch > 1) replayed as one graph
     const int lc = long_ctx(d, pos_h[0]);
     if (!d->exec_fwd[lc]) {
@@ -1082,6 +1089,7 @@ static int decoder_step_argmax_once(thallama_decoder* d, const int* token_h, con
   if (!d || !token_h || !pos_h || !next_h) return (int)hipErrorInvalidValue;
   int r = upload_tok_pos(d, token_h, pos_h);
   if (r) return r;
+  ask_cooperative(d);
   if (d->use_graph && !d->profile) {
     const int lc = long_ctx(d, pos_h[0]);
     if ((r = ensure_greedy_graph(d, lc)) != 0) return r;
@@ -1133,6 +1141,7 @@ static int decoder_greedy_once(thallama_decoder* d, const int* token0_h, const i
     }
   int r = upload_tok_pos(d, token0_h, pos0_h);
   if (r) return r;
+  ask_cooperative(d);
   const bool graph = d->use_graph && !d->profile;
   // step i runs at position pos0 + i: captured before the first replay, one graph per instantiation
   const int lc_first = n_steps > 0 ? long_ctx(d, pos0_h[0]) : 0;

@@ -1139,41 +1139,50 @@ bool persistent_prepare(PStep& p, int ncu, const char** why) {
 // test_give_up_falls_back: a launch missing a block, eager and from a graph).
 // THALLAMA_PERSIST_COOP=0 selects a plain launch (measurement only).  So does a device whose
 // cooperative queue this process cannot have (another process holds it): there a direct launch is
-// refused and a captured one replays without running, so one empty kernel finds out, once per
-// device, before any capture (decoder creation).
+// refused and a captured one replays without running.  One empty kernel finds out, outside any
+// capture, before a decoder's first persistent step: a process that runs none does not take the
+// queue.
 __global__ void k_cooperative_probe() {}
 
-static bool cooperative_queue() {
-  int dev = 0, coop = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&coop, hipDeviceAttributeCooperativeLaunch, dev) != hipSuccess || !coop)
-    return false;
-  ApiLock lock(api_mu());
-  static signed char known[64];  // 1: yes, -1: no
-  if (dev < 64 && known[dev]) return known[dev] > 0;
-  hipStream_t s = nullptr;
-  bool ok = hipStreamCreateWithFlags(&s, hipStreamNonBlocking) == hipSuccess;
-  ok = ok && hipLaunchCooperativeKernel((const void*)k_cooperative_probe, dim3(1), dim3(64), nullptr, 0u, s) == hipSuccess;
-  ok = ok && hipStreamSynchronize(s) == hipSuccess;
-  if (s) (void)hipStreamDestroy(s);
-  if (!ok) (void)hipGetLastError();  // (not sticky for the caller's next launch check)
-  if (dev < 64) known[dev] = ok ? 1 : -1;
-  return ok;
-}
+static signed char g_queue[64];  // by device; 1: this process has it, -1: refused last time (api_mu)
 
-static bool use_cooperative() {
+static bool cooperative_device(int* dev) {
   static const bool off = [] {
     const char* e = getenv("THALLAMA_PERSIST_COOP");
     return e && e[0] == '0';
   }();
-  return !off && cooperative_queue();
+  int coop = 0;
+  return !off && hipGetDevice(dev) == hipSuccess && *dev < 64 &&
+         hipDeviceGetAttribute(&coop, hipDeviceAttributeCooperativeLaunch, *dev) == hipSuccess && coop;
 }
 
-bool persistent_cooperative() { return use_cooperative(); }
+bool persistent_cooperative() {
+  int dev = 0;
+  if (!cooperative_device(&dev)) return false;
+  ApiLock lock(api_mu());
+  return g_queue[dev] >= 0;
+}
+
+bool persistent_cooperative_take() {
+  int dev = 0;
+  if (!cooperative_device(&dev)) return false;
+  ApiLock lock(api_mu());
+  if (g_queue[dev]) return g_queue[dev] > 0;
+  hipStream_t s = nullptr;
+  bool ok = hipStreamCreateWithFlags(&s, hipStreamNonBlocking) == hipSuccess;
+  if (ok) {
+    ok = hipLaunchCooperativeKernel((const void*)k_cooperative_probe, dim3(1), dim3(64), nullptr, 0u, s) == hipSuccess;
+    g_queue[dev] = ok ? 1 : -1;
+    ok = ok && hipStreamSynchronize(s) == hipSuccess;
+    (void)hipStreamDestroy(s);
+  }
+  if (!ok) (void)hipGetLastError();  // (not sticky for the caller's next launch check)
+  return ok;
+}
 
 // The caller zeroes p.sync (kPSyncWords) and the tickets on the same stream right before.
 hipError_t launch_persistent_step(const PStep& p, hipStream_t s, int ncu) {
-  if (use_cooperative()) {
+  if (p.coop) {
     PStep arg = p;
     void* args[] = {&arg};
     return hipLaunchCooperativeKernel(kernel_of(p), dim3(ncu), dim3(PT), args, (unsigned)lds_bytes(p), s);

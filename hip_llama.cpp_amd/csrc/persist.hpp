@@ -50,6 +50,7 @@ struct PStep {
   int B;                    // batched step (persist_b.hip): 2..8 sequences; tok / pos / out and every
                             // hand-off buffer then hold B rows, bmax [grid][8], tickets [L][B*H];
                             // n_scr = the LDS row-chunk partials (persistent_prepare_b)
+  int coop;                 // host: a cooperative launch (persistent_cooperative_take)
   unsigned long long* gk;   // K-split step (persist_k.hip): its hand-off area, persistent_k_granules
                             // granules, zeroed once at allocation
 };
@@ -63,7 +64,11 @@ bool persistent_prepare(PStep& p, int ncu, const char** why);
 // Launch only: the caller zeroes p.sync (kPSyncWords) on stream s right before (a memset
 // node ahead of the kernel node when captured).
 hipError_t launch_persistent_step(const PStep& p, hipStream_t s, int ncu);
-// True if launch_persistent_step uses a cooperative launch (co-residency guaranteed).
+// Can the current device's persistent steps be cooperative launches (co-residency guaranteed), that is, can this
+// process have the device's cooperative queue?  _take finds out, by an empty launch on a stream of its own unless the
+// process has the queue already (not inside a capture); the other one reports without a launch, true where nobody has
+// asked yet.
+bool persistent_cooperative_take();
 bool persistent_cooperative();
 // fp32 batch 1: from this many keys on the step runs the attention helper (persist.hip), so the
 // caller sets PStep::long_ctx and keeps one captured graph per setting

@@ -709,7 +709,7 @@ bool persistent_prepare_b(PStep& p, int ncu, const char** why) {
 // The caller zeroes p.sync and the tickets on the same stream right before (persist.hpp).
 hipError_t launch_persistent_step_b(const PStep& p, hipStream_t s, int ncu) {
   using namespace pb;
-  if (persistent_cooperative()) {
+  if (p.coop) {
     PStep arg = p;
     void* args[] = {&arg};
     return hipLaunchCooperativeKernel(kernel_of(p), dim3(ncu), dim3(PT), args, (unsigned)lds_bytes(p), s);

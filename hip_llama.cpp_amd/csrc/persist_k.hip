@@ -1042,7 +1042,7 @@ hipError_t launch_persistent_step_k(const PStep& p, hipStream_t s, int ncu) {
   PStep arg = p;
   void* args[] = {&arg};
   const unsigned lds = (unsigned)kdyn_bytes(p, ncu);
-  if (persistent_cooperative()) return hipLaunchCooperativeKernel(kernel_of(p), dim3(ncu), dim3(PT), args, lds, s);
+  if (p.coop) return hipLaunchCooperativeKernel(kernel_of(p), dim3(ncu), dim3(PT), args, lds, s);
   return hipLaunchKernel(kernel_of(p), dim3(ncu), dim3(PT), args, lds, s);
 }
 

@@ -53,10 +53,12 @@ enum {
 int thallama_decoder_persistent(thallama_decoder* d);
 /* 1 if that persistent step is the K-split one (8 sequences, THALLAMA_OPT_KSPLIT), else 0. */
 int thallama_decoder_ksplit(thallama_decoder* d);
-/* 1 if the persistent step is dispatched as a cooperative launch (the runtime checks the grid's
- * co-residency; replays of a captured step keep cooperative dispatch on ROCm 7.2 by observation,
- * and every wait is bounded either way), 0 for a plain launch (THALLAMA_PERSIST_COOP=0, no
- * device support, or a device whose cooperative queue another process holds). */
+/* 1 if persistent steps on the current device are dispatched as cooperative launches (the runtime
+ * checks the grid's co-residency; replays of a captured step keep cooperative dispatch on ROCm 7.2
+ * by observation, and every wait is bounded either way), 0 for plain launches
+ * (THALLAMA_PERSIST_COOP=0, no device support, or another process held the device's cooperative
+ * queue when a decoder last asked for it).  A decoder asks before its first persistent step, and
+ * keeps the answer; this call only reports, and launches nothing: 1 where nobody has asked yet. */
 int thallama_persistent_cooperative(void);
 /* Diagnostics: the persistent step's hand-off granules ({value, tag}: x | xb | hb | q k v | int8
  * codes | scales; the last layer's after a launch) into host[n]; returns the count (host NULL:
