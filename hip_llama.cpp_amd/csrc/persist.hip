@@ -1141,7 +1141,7 @@ bool persistent_prepare(PStep& p, int ncu, const char** why) {
 // cooperative queue this process cannot have (another process holds it): there a direct launch is
 // refused and a captured one replays without running.  One empty kernel finds out, outside any
 // capture, before a decoder's first persistent step: a process that runs none does not take the
-// queue.
+// queue.  Once had it stays; a refusal is asked about again by the next decoder.
 __global__ void k_cooperative_probe() {}
 
 static signed char g_queue[64];  // by device; 1: this process has it, -1: refused last time (api_mu)
@@ -1167,7 +1167,7 @@ bool persistent_cooperative_take() {
   int dev = 0;
   if (!cooperative_device(&dev)) return false;
   ApiLock lock(api_mu());
-  if (g_queue[dev]) return g_queue[dev] > 0;
+  if (g_queue[dev] > 0) return true;
   hipStream_t s = nullptr;
   bool ok = hipStreamCreateWithFlags(&s, hipStreamNonBlocking) == hipSuccess;
   if (ok) {

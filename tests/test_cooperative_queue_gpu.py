@@ -1,4 +1,4 @@
-"""GPU: who takes the device's cooperative queue.
+"""GPU: who takes the device's cooperative queue, and what a refusal of it lasts.
 
 One process at a time can have the queue, to its end.  A decoder asks for it before its first persistent step: not at
 creation, not for steps that are no persistent ones, and not when the library is asked for what it knows."""
@@ -48,6 +48,20 @@ def end(p):
     out, err = p.communicate("\n", timeout=60)
     assert p.returncode == 0, err[-3000:]
     return [[int(x) for x in y.split()[1:]] for y in out.splitlines() if y.startswith("tokens")]
+
+
+def test_a_refusal_ends_with_the_holder(gpu, oracle):
+    """A decoder that is refused the queue launches plainly; the next one gets it when the holder has gone."""
+    want = oracle.Model(CFG, 0, seed=5).greedy(1, 0, 8)
+    p = start("decode(1)\nsys.stdin.readline()\n")
+    free = line(p)[2]
+    if not free:
+        end(p)
+        pytest.skip("this process has the cooperative queue, or another one does")
+    q = start("decode(1)\nsys.stdin.readline()\ndecode(1)\n")
+    assert line(q) == [1, 1, 0] + want
+    end(p)
+    assert end(q) == [[1, 1, 1] + want]
 
 
 def test_steps_that_are_not_persistent_leave_the_queue(gpu, oracle):
