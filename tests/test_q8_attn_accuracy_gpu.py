@@ -170,3 +170,20 @@ def test_a_row_of_large_components_leaves_its_neighbours(gpu, handle, B, H, nt):
     rest = [i for i in range(nt) if i not in some]
     np.testing.assert_array_equal(got[:, rest], before[:, rest])
     assert off(got[:, some], before[:, some].astype(np.float64)) < 1e-5  # the keys have nothing there
+
+
+@pytest.mark.parametrize("S,block", [(301, 32), (1400, 128)])
+@pytest.mark.parametrize("mul", [1, 3])
+@pytest.mark.parametrize("hs", [8, 40, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("B,H,nt", FORMS)
+def test_ordinary_rows(gpu, handle, S, block, mul, hs, B, H, nt):
+    """Rows of a normal distribution, whose tokens and channels differ in size, at every number of 64-dimension steps."""
+    if H > 100:  # the card is full from fewer heads on where they are shared
+        H = 130 // mul if hs < 160 else 66 // mul
+        if S > 1000 and hs > 64:
+            S = 700
+    r = rng(hs + S + mul)
+    ref = Cache(B, 1, H, hs, S, block, r)
+    ref.store(0, [0] * B, [S] * B, rows(r, B, S, H, hs), rows(r, B, S, H, hs))
+    q = r.standard_normal((B, nt, H * mul, hs)).astype(np.float32)
+    held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q, "ordinary")

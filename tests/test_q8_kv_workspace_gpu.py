@@ -45,3 +45,28 @@ def test_zeroed_as_documented(gpu, how):
     gpu.sync()
     hold(out.download().reshape(q.shape), want, bound, how)
     assert dev.lib.thablasDestroy(handle) == 0
+
+
+def test_one_workspace_for_calls_of_any_shape(gpu, handle):
+    """Calls of differing heads, rows and lengths, ragged and full, one after another on one workspace of the documented
+    size: each agrees with the reference, and nothing behind the workspace is written."""
+    r = rng(11)
+    B, H, hs, S = 3, 4, 64, 5000
+    ref, dev = filled(gpu, handle, r, B, 1, H, hs, S, 64, [S] * B, 0)
+    size = dev.lib.thaDNN_q8_attention_workspace(C.byref(dev.c), 1, 1, H)
+    guard = 1 << 16
+    work = gpu.DevBuf(size + guard)
+    work.upload(np.concatenate([np.zeros(size, np.uint8), np.full(guard, 0xA5, np.uint8)]))
+    shapes = [(1, 1, 1, [4999]), (3, 5, 2, [4000, 17, 2500]), (2, 1, 8, [4999, 300]), (3, 70, 1, [4000, 4100, 0]), (1, 3, 1, [100]),
+              (3, 1, 1, [4999, 4998, 64]), (2, 40, 4, [3000, 1]), (1, 1, 2, [4999]), (3, 300, 2, [1000, 0, 4700])]
+    for nb, nt, mul, pos in shapes * 2:
+        q = r.standard_normal((nb, nt, H * mul, hs)).astype(np.float32)
+        p, dq = dev.ints(pos), gpu.DevBuf.from_array(q)
+        out = gpu.DevBuf.from_array(np.full(q.size, -77.0, np.float32))
+        assert dev.lib.thaDNN_q8_attention_batch(C.byref(handle), C.byref(dev.c), 0, nb, nt, p.ptr, None, H * mul, dq.ptr, out.ptr, H * mul * hs,
+                                                 H * mul * hs, work.ptr, size) == 0
+        gpu.sync()
+        some = sorted({0, nt // 2, nt - 1})
+        want, bound = ref.attend(0, pos, [nt] * nb, nt, q, mul, some)
+        hold(out.download().reshape(q.shape)[:, some], want[:, some], bound[:, some], f"{nb} x {nt} x {mul}")
+        assert (work.download(np.uint8, guard, size) == 0xA5).all()
