@@ -52,7 +52,7 @@ struct Q8AttnArgs {
   unsigned* arrived;  // nsplit > 1: [unit] workgroups that have left their part; 0 between calls
   float* part;        // nsplit > 1: [unit][split][lrows][head_size rounded up to 4, + 4]
   long long q_stride, out_stride;
-  int n_heads, mul;  // query heads, and how many of them share a K/V head
+  int mul;           // query heads that share a K/V head
   int tiles;         // row tiles of a (sequence, K/V head)
   int nsplit;        // workgroups that share a row tile's keys
   int lrows;         // rows of a tile that any sequence can have
@@ -983,7 +983,6 @@ extern "C" thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, co
   a.part = reinterpret_cast<float*>(a.arrived + tl::kAttnUnits * tl::kCountStep);
   a.q_stride = q_stride;
   a.out_stride = out_stride;
-  a.n_heads = n_heads;
   a.mul = mul;
   a.tiles = (int)p.tiles;
   a.nsplit = p.nsplit;
