@@ -40,7 +40,6 @@ constexpr float kRound = 8421504.f;   // 2^23 + 0x8080: a sum with it is rounded
 constexpr float kNone = -3.4e38f;     // a maximum over nothing
 constexpr float kLag = 16.f;          // log2 of how far a step's maximum may be past the sums' unit
 constexpr int kUnit = 28;             // power of two in c0, so that its product with a key scale is a normal float
-constexpr float kFew = 0x1p26f;       // sums of a row under this many of a step's units: its weights' further digits count
 constexpr int kWaves = 4;             // of a workgroup
 constexpr int kCountStep = 32;        // a cache line for each count of arrivals
 
@@ -445,8 +444,11 @@ TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, co
   attn_values<KS, NT>(s.o, p, beta, val);
 
   // Too few digits?  Half a unit for each n_t of 64 to 256 keys, of codes up to 127 and about 30 in the mean, is some 50 to
-  // 130 units beside the row's sums, which are about 2^28 where one key's ordinary codes are all that counts.  Looked at in
-  // the first 32 dimensions, or 16 of fewer; lanes whose four of these go past the head's end have no say.
+  // 130 units beside the row's sums, which are about 2^28 where one key's ordinary codes are all that counts: few are under
+  // 2^25.5 to 2^26 units.  (2^26 at heads of 128 costs calls of one round of workgroups an eighth, 352 tiles of 64 rows 24.4
+  // us for 22.7, where blocks with a large token leave the others small codes.)  Looked at in the first 32 dimensions, or 16
+  // of fewer; lanes whose four of these go past the head's end have no say.
+  constexpr float kFew = KS == 1 ? 0x1p26f : 0x1.6ap25f;
   const float second = KS > 1 || a.l.head_size >= 32 ? 1.f : 0.f;
   float most = 0.f;
 #pragma unroll
