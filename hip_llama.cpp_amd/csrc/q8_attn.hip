@@ -181,8 +181,9 @@ struct AttnMore {
 };
 
 // The query's digits.  True if they are too few for the row: where a few components are so much larger than the rest that
-// these have few of the 24 bits.  Goes by the mean of every other eight components, none taken for more than 2^-4 of the
-// largest number: under 3/8 of that where the largest component is past some 34 times the width of the others' distribution.
+// these have few of the 24 bits.  Goes by the mean of eight of each sixteen components, none taken for more than 2^-5 of the
+// largest number, so that up to half of them may be large: under 0.6 of that where the largest component is past some 34 times the width of
+// the others' distribution.
 template <int KS>
 TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen) {
   s.seen = seen;
@@ -196,7 +197,7 @@ TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
   s.qn = top < 0x7f800000u ? 1.f : __builtin_nanf("");
   const int qe = top < 0x7f800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
   s.qe = qe - kUnit;
-  constexpr float most = kDigits / 16.f;
+  constexpr float most = kDigits / 32.f;
   float size = 0.f;
 #pragma unroll
   for (int k = 0; k < KS; ++k)
@@ -215,7 +216,7 @@ TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
       s.q[1][k][e] = p1;
       s.q[2][k][e] = p2;
     }
-  return rows_sum(size) < 0.375f * most * (float)((hs >> 4) * 8 + min(hs & 15, 8)) && top > 0u && top < 0x7f800000u;
+  return rows_sum(size) < 0.6f * most * (float)((hs >> 4) * 8 + min(hs & 15, 8)) && top > 0u && top < 0x7f800000u;
 }
 
 // Scales of this lane's sixteen keys in each of NT tiles of 64 from t0 on; behind the last key those of its block.

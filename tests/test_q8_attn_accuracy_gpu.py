@@ -151,6 +151,22 @@ def test_queries_of_a_few_large_components(gpu, handle, size, count, keys, hs, B
     held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q.astype(np.float32), f"{count} of {size}, keys times {keys}")
 
 
+@pytest.mark.parametrize("size", [200, 2e4])
+@pytest.mark.parametrize("hs,large", [(8, [0, 1, 5]), (16, [0, 2, 3]), (16, [1, 3, 7]), (24, [0, 1, 2, 17]), (40, [0, 1, 2, 3, 4, 5, 6])])
+@pytest.mark.parametrize("B,H,nt", FORMS)
+def test_small_heads_of_large_components(gpu, handle, size, hs, large, B, H, nt):
+    """The same where the large components are a good part of a small head's."""
+    r = rng(nt + hs + len(large))
+    S = 300
+    k, v = r.standard_normal((B, S, H, hs)), r.standard_normal((B, S, H, hs))
+    q = r.standard_normal((B, nt, H, hs))
+    q[..., large] = size
+    k[..., large] = 0
+    ref = Cache(B, 1, H, hs, S, 32, r)
+    ref.store(0, [0] * B, [S] * B, k.astype(np.float32), v.astype(np.float32))
+    held(gpu, handle, ref, [S - nt - 7 * b for b in range(B)], q.astype(np.float32), f"{large} of {size}")
+
+
 @pytest.mark.parametrize("B,H,nt", FORMS[1:])
 def test_a_row_of_large_components_leaves_its_neighbours(gpu, handle, B, H, nt):
     """Rows whose queries need more digits do not change a bit of the rows beside them."""
