@@ -13,12 +13,13 @@
 // sv = f 2^e, 1/2 <= f < 1, and E the row's largest e so far, the running maximum M is taken of y_t = x_t + (e_t - E) (as
 // exact as x_t itself, whatever the values' size), u_t = 2^(y_t - M) is at most 1 and n_t = u_t f_t 0x7f7f7f.  The sum of
 // the weights adds u_t 2^(E - e_t); value scales under 2^(E - 40) count as that e with a smaller f, so that u_t cannot
-// vanish where its weight does not; a row is so off by up to 2^-64 of 127 of the largest value scale in sight, too.  M is the maximum of one step's 64 to 256 keys, so that a
-// large weight elsewhere costs the step's own no digits; the steps are summed in fp32, in units of a power that follows
-// M only where it rises past 2^16 of it.  A large weight on a key of small values still costs its neighbours theirs (the
-// first token of a model, with nearly all of a row's weight and nothing in its values: without more, the row would be 4e-5 to 1e-1
-// off): where a step leaves a row's sums small its weights get three more digits behind these.  Against 64 bits the shapes named at the kernels are 3e-7 to 7e-7 off (2-norm),
-// an fp32 softmax over the same codes 3e-7 to 1.8e-6.
+// vanish where its weight does not; a row is so off by up to 2^-64 of 127 of the largest value scale in sight, too.  M is
+// the maximum of one step's 64 to 256 keys, so that a large weight elsewhere costs the step's own no digits; the steps are
+// summed in fp32, in units of a power that follows M only where it rises past 2^16 of it.  A large weight on a key of
+// small values still costs its neighbours theirs (a model's first token, with nearly all of a row's weight and nothing in
+// its values: the row would be 4e-5 to 1e-1 off): where a step leaves a row's sums small its weights get three more digits
+// behind these.  Against 64 bits the shapes named at the kernels are 5e-7 to 7e-7 off (2-norm), an fp32 softmax over the
+// same codes 2e-7 to 1.8e-6; with such a key in each row, or a large component in each query, both 2e-7 to 2e-6.
 //
 // The int8 cores' peak is 5 POP/s beside 157 TFLOP/s for fp32 inputs, so three products are still ten times as fast as
 // one in fp32, and the cache is read as it is, without a conversion.
@@ -399,7 +400,7 @@ TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, co
   f4 x[NT][4];
   attn_scores<KS, NT>(x, c, s, more, a, edge, left, key);
   const float m = attn_most<NT>(x);  // of this step alone: it sets the size that the step's weights are rounded to
-  // Rare behind the first step (four prompts of 2048 tokens, 32 heads of 128: 272 us; scaled in each step 276).
+  // Rare behind the first step (four prompts of 2048 tokens, 32 heads of 128: 278 us; scaled in each step 282).
   const float M = m - kLag > s.M ? __builtin_ceilf(m) : s.M;  // whole, so that it moves by grow without a rounding
   if (__any(M != s.M || grow)) {
     const float alpha = __builtin_amdgcn_exp2f(s.M - M);
@@ -480,7 +481,8 @@ struct AttnMarks {
 // What a step's weights have beyond their 24 bits: u_t f_t 0x7f7f7f - n_t, at most 1/2, in three more digits of 2^-24 each.
 // A row needs it where one key has far more weight than others and next to nothing in its values (a model's first token),
 // in the steps that hold such a key.  Its operands are read again when all keys are through, and taken tile by tile: in the
-// loop itself the registers would be short.
+// loop itself the registers would be short.  With such a first key in every row: one row of 32 heads over 2048 keys 9.1 ->
+// 9.9 us, eight to 32768 keys 65.8 -> 68.3, four prompts 278 -> 327.
 template <int KS, int NT, bool WIDE>
 TL_DEVICE void attn_further(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, const AttnHead& h, int t0, bool edge, bool mine) {
   int lane = threadIdx.x & 63;
@@ -561,7 +563,7 @@ TL_DEVICE AttnMore<KS, true> attn_more(const AttnRows<KS>& s, const Q8AttnArgs& 
 }
 
 // A wave's keys, its steps of 64 from key `from` on `step` apart, with six digits of the queries that want them (`mine`).
-// Rare, and plain.
+// Rare, and plain: one row of 32 heads over 2048 keys 9.1 -> 15.4 us, four prompts 278 -> 1216 where every row wants them.
 template <int KS>
 TL_DEVICE void attn_wide(AttnRows<KS>& s, const Q8AttnArgs& a, const AttnUnit& w, const AttnHead& h, int r0, bool mine, int from, int step, int least) {
   int lane = threadIdx.x & 63;
@@ -647,7 +649,7 @@ TL_DEVICE void lds_wait() {
 }
 
 // A tile of 64 keys as one wave holds it.  ONCE: no other row tile reads these codes, and they need not stay in L2 (kept
-// there, eight rows over 10923 to 32768 keys take 71.5 us for 65.5; not kept, 256 rows of 32 heads over 16640 keys,
+// there, eight rows over 10923 to 32768 keys take 73.7 us for 65.8; not kept, 256 rows of 32 heads over 16640 keys,
 // sixteen tiles a head, 228 for 167).
 template <int KS, bool ONCE>
 struct AttnTile {
@@ -675,9 +677,9 @@ struct AttnTile {
 // its next values when the sums are.  The waves' results are joined in LDS; where several workgroups share a row tile,
 // each leaves its result in the workspace and the last one to arrive joins them, in the order of the splits whoever it is.
 //
-// Long contexts are bound by memory: eight rows of 32 heads over 8 K/V heads of 128 at 10923 to 32768 keys 65.5 us,
-// 5.5 TB/s of codes (the vector pipe 30% busy), sixteen rows of 32 heads at 683 to 2048 keys 34 us, 5.2 TB/s.  Short ones
-// are bound by a chain of latencies: positions, keys, two products and the joins, 12 heads of 64 over 301 keys 5.8 us, 32
+// Long contexts are bound by memory: eight rows of 32 heads over 8 K/V heads of 128 at 10923 to 32768 keys 65.8 us,
+// 5.4 TB/s of codes (the vector pipe 27% busy), sixteen rows of 32 heads at 683 to 2048 keys 34.6 us, 5.2 TB/s.  Short ones
+// are bound by a chain of latencies: positions, keys, two products and the joins, 12 heads of 64 over 301 keys 6.1 us, 32
 // of 128 over 2048 keys 9.1 (0.8 until the positions are there, 2.7 to the first codes, 2 for a tile, 0.9 to join the
 // waves, 2.5 the workgroups).
 template <int KS, bool ONCE>
@@ -802,11 +804,11 @@ __global__ void __launch_bounds__(256, KS == 1 ? 4 : KS < 4 ? 2 : 1) k_q8_attn_f
 // chunk's keys while the values are.  LDS holds the codes in the order in which the lanes want them, one KiB for
 // each operand of a product, so that a load (16 bytes a lane, memory to LDS) and a read are both linear in the lane.
 //
-// Bound by vector instructions and by power: 64 keys x 16 rows at heads of 128 take a SIMD 2070 cycles, of which 370
-// vector instructions fill 1660 and 48 products, beside them, 768.  Four 2048-token prompts of 32 heads: 272 us, 505
-// TFLOP/s of attention (three times that in int8 operations), the vector pipe 84% busy at the 1.94 GHz that the card
-// holds under this load.  Two tiles a step leave room for three waves on a SIMD (343 us, four tiles and two waves 352, on
-// one card), heads of 64 fit three with four.
+// Bound by vector instructions and by power: 64 keys x 16 rows at heads of 128 take a SIMD 2100 cycles, of which 363
+// vector instructions and 48 products fill 1720, and the products, beside them, 768.  Four 2048-token prompts of 32 heads:
+// 272 to 280 us by the card, 491 to 505 TFLOP/s of attention (three times that in int8 operations), the vector pipe 80%
+// busy at the 1.92 GHz that the card holds under this load.  Two tiles a step leave room for three waves on a SIMD (2%
+// faster than four tiles and two waves), heads of 64 fit three with four.
 template <int KS, int NT>
 __global__ void __launch_bounds__(256, KS < 3 ? 3 : 2) k_q8_attn_many(Q8AttnArgs a) {
   keep_implicit_args();  // common.hpp
@@ -903,16 +905,16 @@ struct AttnPlan {
 static AttnPlan attn_plan(const Q8KVCache* c, int n_batches, int n_tokens, int n_heads) {
   AttnPlan p;
   const long long rows = (long long)n_tokens * (n_heads / c->n_kv_heads), pairs = (long long)n_batches * c->n_kv_heads;
-  // Tiles of 64 rows that fill the card go to k_q8_attn_many: from 256 of them on (256, of 32 heads x 512 rows: 16.5 us,
-  // k_q8_attn_few 19.1; 224: 15.1 and 16.1; 352: 22.4 and 28.6), at heads of up to 64, where the few rows' kernel fits
-  // four waves on a SIMD, from 512 (264, of 12 heads x 1400 rows: 24.0 us and 17.3; 528, of two
-  // sequences: 26.5 and 27.5).
+  // Tiles of 64 rows that fill the card go to k_q8_attn_many: from 256 of them on (256, of 32 heads x 512 rows: 16.7 us,
+  // k_q8_attn_few 19.8; 224: 17.0 and 18.0; 352: 22.7 and 28.7), at heads of up to 64, where the few rows' kernel fits
+  // four waves on a SIMD, from 512 (264, of 12 heads x 1400 rows: 24.4 us and 16.6; 528, of two
+  // sequences: 26.3 and 27.7).
   p.many = rows >= 64 && pairs * ((rows + 63) / 64) >= (c->head_size <= 64 ? 2 : 1) * kAttnUnits;
   p.tiles = p.many ? (rows + 63) / 64 : (rows + 15) / 16;
   p.units = pairs * p.tiles;
   // The keys of few tiles are divided until there is a workgroup for each CU, but no further than each wave has a tile (one
-  // row of 32 heads over 2048 keys: 9.1 us), or two for each CU where each wave still has eight and no other row tile
-  // reads the same keys at its own pace (eight rows of 8 K/V heads over 10923 to 32768 keys: 66 us, with one 73; 32 rows
+  // row of 32 heads over 2048 keys: 9.1 us, divided twice as far 10.7), or two for each CU where each wave still has eight and no other row tile
+  // reads the same keys at its own pace (eight rows of 8 K/V heads over 10923 to 32768 keys: 66 us, with one 72; 32 rows
   // of 32 heads over 16416, two tiles a head: 46 us, with one 34).
   const long long most = (c->seq_len + 64LL * kWaves - 1) / (64 * kWaves);
   p.nsplit = p.many ? 1 : (int)max(1LL, min(most, min((long long)kMaxSplit, kAttnUnits / p.units)));
