@@ -182,9 +182,9 @@ struct AttnMore {
 };
 
 // The query's digits.  True if they are too few for the row: where a few components are so much larger than the rest that
-// these have few of the 24 bits.  Goes by the mean of eight of each sixteen components, none taken for more than 2^-5 of the
-// largest number, so that up to half of them may be large: under 0.6 of that where the largest component is past some 34 times the width of
-// the others' distribution.
+// these have few of the 24 bits.  Goes by the mean of some of each sixteen components, none taken for more than 2^-5 of the
+// largest number, so that up to half of them may be large, and zeros, which need no bits, for as much: under 0.6 of that
+// where the largest component is past some 34 times the width of the others' distribution.
 template <int KS>
 TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen) {
   s.seen = seen;
@@ -199,6 +199,7 @@ TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
   const int qe = top < 0x7f800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
   s.qe = qe - kUnit;
   constexpr float most = kDigits / 32.f;
+  constexpr int kSome = KS == 1 ? 8 : 4;
   float size = 0.f;
 #pragma unroll
   for (int k = 0; k < KS; ++k)
@@ -208,7 +209,7 @@ TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float y = __builtin_ldexpf(x[k][4 * e + c], -qe) * kDigits;
-        if (e < 2) size += fminf(fabsf(y), most);
+        if (4 * e < kSome) size += __uint_as_float(min((__float_as_uint(y) & 0x7fffffffu) - 1u, __float_as_uint(most)));
         n[c] = (unsigned)(int)rintf(y) + 0x8080u;
       }
       int p0, p1, p2;
@@ -217,7 +218,8 @@ TL_DEVICE bool attn_begin(AttnRows<KS>& s, float (&x)[KS][16], int hs, int seen)
       s.q[1][k][e] = p1;
       s.q[2][k][e] = p2;
     }
-  return rows_sum(size) < 0.6f * most * (float)((hs >> 4) * 8 + min(hs & 15, 8)) && top > 0u && top < 0x7f800000u;
+  // with the zeros behind the head's end
+  return rows_sum(size) < most * (4.f * KS * kSome - 0.4f * (float)((hs >> 4) * kSome + min(hs & 15, kSome))) && top - 1u < 0x7f7fffffu;
 }
 
 // Scales of this lane's sixteen keys in each of NT tiles of 64 from t0 on; behind the last key those of its block.
@@ -379,7 +381,8 @@ struct AttnHead {
 // One step of NT tiles of 64 keys from t0 on; key and val as above.  ready() runs between the two products.  The rows of
 // the wave whose weights need further digits, as bits.
 template <int KS, int NT, bool WIDE, class Key, class Val, class Ready>
-TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val, Ready ready) {
+TL_DEVICE unsigned attn_step(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, AttnScales<NT>& c, int t0, bool edge, Key key, Val val,
+                             Ready ready) {
   constexpr int DT = 4 * KS;
   const int g = (threadIdx.x & 63) >> 4;
   const int left = s.seen - t0 - 16 * g;  // keys of this lane's first tile and behind it that the row sees
@@ -527,7 +530,8 @@ TL_DEVICE void attn_further(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, con
 }
 // The marked ones of a wave's steps 0 .. last, that of number i from key from + i * step on.
 template <int KS, int NT, bool WIDE>
-TL_DEVICE void attn_marked(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, const AttnHead& h, const AttnMarks& marks, int from, int step, int last, int least) {
+TL_DEVICE void attn_marked(AttnRows<KS>& s, const AttnMore<KS, WIDE>& more, const Q8AttnArgs& a, const AttnHead& h, const AttnMarks& marks, int from, int step,
+                           int last, int least) {
   if (__builtin_expect(!__any(marks.bits), 1)) return;
 #pragma unroll 1
   for (int i = 0; i <= last; ++i) {

@@ -69,16 +69,16 @@ size_t thaDNN_q8_attention_workspace(const Q8KVCache* c, int n_batches, int n_to
 //   out_i[h] = sum_{t <= p} softmax_t(q_i[h] . k_t / sqrtf(head_size)) v_t,   p = pos_d[b] + i
 // in fp32's accuracy: q is taken to 2^-24 of its row's largest component, and to 2^-47 where that is past some 34 times the
 // others; a weight times its value block's scale to 2^-24 of the largest such product among up to 256 keys around it, and to
-// 2^-48 of it where the row's sums are under 8 to 16 times that product (so that a key of most of the weight and of small
+// 2^-48 of it where the row's sums are under 6 to 16 times that product (so that a key of most of the weight and of small
 // values costs the others no accuracy); or to 2^-64 of the largest scale, if that is more.
 // A decode step is n_tokens = 1 after its token's store, a prompt's chunk n_tokens > 1.
 // A row at a position outside 0 .. seq_len - 1 sees no key: zeros.  Rows from n_d[b] on are left as they were.
 // q and out are [n_batches][n_tokens][n_heads * head_size] and do not overlap.  work (16-byte aligned) is zeroed once,
-// before its first call, and then left to these calls, of any shape: each leaves it ready for the next.  The zeroing is done
-// before that call's kernel runs: by thallama_memset, which waits for it, or by hipMemsetAsync on handle->calc_stream, outside
-// any capture (a plain hipMemset is not ordered before that stream).  It
-// belongs to a call until its kernel has run: calls that may run at once, captured ones among them, have one each.  A
-// call during which pos_d or n_d change leaves it to be zeroed again.
+// before its first call, and then left to these calls, of any shape: each leaves it ready for the next.  The zeroing is
+// done before that call's kernel runs: by thallama_memset, which waits for it, or by hipMemsetAsync on
+// handle->calc_stream, outside any capture (a plain hipMemset is not ordered before that stream).  work belongs to a call
+// until its kernel has run: calls that may run at once, captured ones among them, have one each.  A call during which
+// pos_d or n_d change leaves it to be zeroed again.
 thablasStatus_t thaDNN_q8_attention_batch(thablasHandle_t* handle, const Q8KVCache* c, int layer, int n_batches,
                                           int n_tokens, const int* pos_d, const int* n_d, int n_heads,
                                           const float* q, float* out, int q_stride, int out_stride, void* work,
