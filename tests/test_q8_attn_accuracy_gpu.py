@@ -11,7 +11,7 @@ at most, and half as much again is for the few rows of a call.
 integers: a weight times its value block's scale is n 2^-23 of its step's largest w_t 2^e_t, and the scale at least half of
 2^e_t: off by up to half of 2^-22 of the largest weight times scale, 2^-22 / sqrt(12) in the mean.  A step has up to 256
 keys of about the same codes: sqrt(256) 2^-22 / sqrt(12) = 1.1e-6 of what the largest key itself adds to the row, and the
-row is no smaller than that where the values are of one size (where it is, the weights have more digits)."""
+row is no smaller than that where the values are of one size; where it is smaller, the weights have more digits."""
 import numpy as np
 import pytest
 
